@@ -18,6 +18,7 @@ LIB_PATH = os.path.join(HERE, "librv12.so")
 RV12_OK = 0
 RV12_E_NULL, RV12_E_SHAPE, RV12_E_MODE, RV12_E_TOKENS = -1, -2, -3, -4
 RV12_E_WORKSPACE, RV12_E_CONFIG, RV12_E_BASE, RV12_E_ALIGN, RV12_E_SIZE, RV12_E_SCRATCH = -5, -6, -7, -8, -9, -10
+RV12_E_PAGED = -11
 RV12_E_LAUNCH = -20
 
 # every symbol include/rv12.h declares
@@ -29,7 +30,8 @@ EXPORTS = ("rv12_abi_version", "rv12_strerror", "rv12_tiles_bytes", "rv12_pack_p
            "rv12_prefill_rope_attn", "rv12_prefill_workspace_bytes",
            "rv12_prefill_linear", "rv12_decode_advance",
            "rv12_compress_workspace_bytes", "rv12_compress_plan", "rv12_compress_write",
-           "rv12_prefill_parts_workspace_bytes", "rv12_prefill_linear_parts")
+           "rv12_prefill_parts_workspace_bytes", "rv12_prefill_linear_parts",
+           "rv12_paged_append", "rv12_paged_attend_workspace_bytes", "rv12_paged_attend")
 ABI_VERSION = 8
 STATIC_SCRATCH_BYTES = 8 << 20  # RV12_STATIC_SCRATCH_BYTES
 
@@ -58,6 +60,13 @@ KERNEL_VECTOR, KERNEL_MFMA, KERNEL_MFMA_KSPLIT = 1, 2, 3
 class Attn(ctypes.Structure):
     _fields_ = [("n_heads", ctypes.c_int32), ("n_kv", ctypes.c_int32), ("head_dim", ctypes.c_int32),
                 ("maxt", ctypes.c_int32), ("kv_bf16", ctypes.c_int32), ("splits", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("scale", ctypes.c_float)]
+
+
+class Paged(ctypes.Structure):
+    _fields_ = [("n_heads", ctypes.c_int32), ("n_kv", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("page", ctypes.c_int32), ("kv_bf16", ctypes.c_int32), ("n_seq", ctypes.c_int32),
+                ("max_pages", ctypes.c_int32), ("table_stride", ctypes.c_int64), ("n_pages", ctypes.c_int64),
                 ("eps", ctypes.c_float), ("scale", ctypes.c_float)]
 
 
@@ -145,6 +154,12 @@ def lib():
         L.rv12_prefill_attn_workspace_bytes.argtypes = [ctypes.POINTER(Attn), I]
         L.rv12_prefill_rope_attn.restype = I
         L.rv12_prefill_rope_attn.argtypes = [ctypes.POINTER(Attn), I, P, P, P, P, P, P, P, P, P, SZ, P]
+        L.rv12_paged_append.restype = I
+        L.rv12_paged_append.argtypes = [ctypes.POINTER(Paged), I, P, P, P, P, P, P, P, P, P, P, P]
+        L.rv12_paged_attend_workspace_bytes.restype = SZ
+        L.rv12_paged_attend_workspace_bytes.argtypes = [ctypes.POINTER(Paged), I]
+        L.rv12_paged_attend.restype = I
+        L.rv12_paged_attend.argtypes = [ctypes.POINTER(Paged), I, P, P, P, P, P, P, P, P, SZ, P]
         v = L.rv12_abi_version()
         if v != ABI_VERSION:
             raise RuntimeError(f"librv12.so ABI version {v}, expected {ABI_VERSION}")

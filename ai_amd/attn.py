@@ -6,12 +6,20 @@ tokens of one sequence, each attending causally (rv12_rope_attn_batch: the
 reference's qk_rope_cache_k + attn_k, tkernels.py:82-150), or a whole prompt
 block (rv12_prefill_rope_attn: qk_rope_cache_k + att_k of the blocked prefill,
 ramvi/engine/ramvi_engine/kernels/prefill.py:100-103,
-prefill_kernels.py:29-54)."""
+prefill_kernels.py:29-54).  Many sequences share a cache in pages
+(PagedRopeAttn: rv12_paged_append, rv12_paged_attend)."""
 import ctypes
 
 import torch
 
-from ._lib import Attn, check, lib
+from ._lib import Attn, Paged, check, lib
+from .wcomp import _ptr, _stream
+
+
+def _on(dev):
+    """The device of a call's tensors as the current one: a launch goes to the
+    current device, whatever its stream."""
+    return torch.cuda.device(dev)
 
 
 SPAN = 80  # positions one workgroup covers at most
@@ -108,3 +116,113 @@ class RopeAttn:
                                       p(vc), p(out), p(ws), ws.numel(),
                                       ctypes.c_void_p(torch.cuda.current_stream(qkv.device).cuda_stream))
         check(rc, "prefill_rope_attn")
+
+
+class PagedRopeAttn:
+    """Attention over a cache of many sequences in pages (rv12_paged_append,
+    rv12_paged_attend).  A pass has T token rows; row r is position pos[r] of
+    sequence seq[r].  Rows may be of different sequences (one new token each) or
+    of one (a chunk of its prompt, speculated tokens), in any order; those of
+    one sequence run faster next to each other.  The tensors of a call, all on
+    one GPU, contiguous but for the table's rows:
+
+        qkv    float32 [T, (n_heads + 2 n_kv) head_dim], the qkv linear's output
+        q, out float32 [T, n_heads head_dim]
+        seq    int32 [T], or None: row r is of sequence r
+        pos    int64 [T]
+        table  int32 [sequences, pages of one], the page ids of each sequence
+               (any stride between its rows)
+        kc, vc [pages, n_kv, page, head_dim] of kv_dtype
+
+    A row with seq or pos outside the table (-1 for padding a pass to a fixed
+    size) is padding: its q and out are zeros and it writes nothing.  A page id
+    outside the cache (-1) is no page: its positions take no part in the
+    attention, a key or value for it is dropped.  Rows that name one slot
+    together leave it with either's key and value.  seq, pos and table are read
+    on the device, so a call can be captured in a HIP graph; every call has a
+    workspace of its own.  The rotation angle is formed in 64 bits (RopeAttn's
+    in float32: the two agree to float32 rounding times the position)."""
+
+    def __init__(self, n_heads, n_kv, head_dim, page, kv_dtype, eps, scale=None):
+        if kv_dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("the cache must be float32 or bfloat16")
+        self.kv_dtype = kv_dtype
+        self.n_heads, self.n_kv, self.head_dim, self.page = (int(v) for v in (n_heads, n_kv, head_dim, page))
+        self.eps = float(eps)
+        self.scale = float(self.head_dim ** -0.5 if scale is None else scale)
+        a = self._struct(1, 1, 1, 1)
+        if lib().rv12_paged_attend_workspace_bytes(ctypes.byref(a), 1) == 0:
+            raise ValueError("paged attention: head_dim must be 64 or 128, n_heads 1 to 16 times n_kv, page a power of "
+                             "two from 16 to 1024")
+
+    def _struct(self, n_seq, max_pages, stride, n_pages):
+        return Paged(self.n_heads, self.n_kv, self.head_dim, self.page, 1 if self.kv_dtype == torch.bfloat16 else 0,
+                     n_seq, max_pages, stride, n_pages, self.eps, self.scale)
+
+    def _rows(self, rows, seq, pos, table, kc, vc):
+        """The argument struct of a call and its row count; rows: (tensor,
+        floats of one row) pairs."""
+        first = rows[0][0]
+        if not first.is_cuda:
+            raise ValueError("the tensors must be on the GPU")
+        dev = first.device
+        T = pos.numel()
+        if pos.dtype != torch.int64 or pos.dim() != 1 or not pos.is_contiguous() or pos.device != dev:
+            raise ValueError("pos must be a contiguous int64 vector on the rows' device")
+        if seq is not None and (seq.dtype != torch.int32 or seq.shape != pos.shape or not seq.is_contiguous()
+                                or seq.device != dev):
+            raise ValueError("seq must be an int32 vector with an entry for every row, on the rows' device")
+        for t, n in rows:
+            if t.dtype != torch.float32 or not t.is_contiguous() or t.device != dev or t.numel() != T * n:
+                raise ValueError(f"qkv, q and out must be contiguous float32 with {T} rows, on one device")
+        if (table.dtype != torch.int32 or table.dim() != 2 or table.device != dev or table.stride(1) != 1
+                or min(table.shape) < 1):
+            raise ValueError("table must be int32 [sequences, pages], its rows contiguous, on the rows' device")
+        for c in (kc, vc):
+            if (c.dtype != self.kv_dtype or not c.is_contiguous() or c.device != dev or c.dim() != 4
+                    or tuple(c.shape[1:]) != (self.n_kv, self.page, self.head_dim) or c.shape != kc.shape):
+                raise ValueError(f"kc and vc must be contiguous {self.kv_dtype} caches of shape "
+                                 f"(pages, {self.n_kv}, {self.page}, {self.head_dim})")
+        n_seq, max_pages = table.shape
+        stride = table.stride(0) if n_seq > 1 else max_pages
+        if stride < max_pages:
+            raise ValueError("the table's rows must not overlap")
+        return self._struct(n_seq, max_pages, stride, kc.shape[0]), T
+
+    def append(self, qkv, qn, kn, inv, seq, pos, table, kc, vc, q):
+        """Head norms and rotation of the rows' q and k: q to q, k and v to
+        their pages."""
+        a, T = self._rows([(qkv, (self.n_heads + 2 * self.n_kv) * self.head_dim), (q, self.n_heads * self.head_dim)],
+                          seq, pos, table, kc, vc)
+        for t, n in ((qn, self.head_dim), (kn, self.head_dim), (inv, self.head_dim // 2)):
+            if t.dtype != torch.float32 or not t.is_contiguous() or t.device != qkv.device or t.numel() != n:
+                raise ValueError("qn, kn and inv must be contiguous float32 of head_dim, head_dim and head_dim / 2 "
+                                 "entries, on the rows' device")
+        if T == 0:
+            return
+        with _on(qkv.device):
+            check(lib().rv12_paged_append(ctypes.byref(a), T, _ptr(qkv), _ptr(qn), _ptr(kn), _ptr(inv), _ptr(seq),
+                                          _ptr(pos), _ptr(table), _ptr(kc), _ptr(vc), _ptr(q), _stream(qkv.device)),
+                  "paged_append")
+
+    def attend(self, q, seq, pos, table, kc, vc, out):
+        """The attention of the rows (q as append leaves it) over their
+        sequences' positions 0 .. pos, the rows' own among them."""
+        n = self.n_heads * self.head_dim
+        a, T = self._rows([(q, n), (out, n)], seq, pos, table, kc, vc)
+        if T == 0:
+            return
+        L = lib()
+        with _on(q.device):
+            need = L.rv12_paged_attend_workspace_bytes(ctypes.byref(a), T)
+            if need == 0:
+                raise ValueError("paged attention: too many rows or positions")
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+            check(L.rv12_paged_attend(ctypes.byref(a), T, _ptr(q), _ptr(seq), _ptr(pos), _ptr(table), _ptr(kc),
+                                      _ptr(vc), _ptr(out), _ptr(ws), need, _stream(q.device)), "paged_attend")
+
+    def __call__(self, qkv, qn, kn, inv, seq, pos, table, kc, vc, out):
+        """append, then attend."""
+        q = torch.empty_like(out)
+        self.append(qkv, qn, kn, inv, seq, pos, table, kc, vc, q)
+        self.attend(q, seq, pos, table, kc, vc, out)

@@ -379,6 +379,9 @@ const char* rv12_strerror(int s) {
         case RV12_E_ALIGN: return "x, y, lnw or tiles not aligned (16 bytes; lnw 8 bytes)";
         case RV12_E_SIZE: return "tiles buffer smaller than rv12_tiles_bytes()";
         case RV12_E_SCRATCH: return "workspace of the launch exceeds the static scratch (RV12_STATIC_SCRATCH_BYTES, 8 MiB)";
+        case RV12_E_PAGED:
+            return "bad paged cache or rows (head_dim 64 or 128, up to 16 query heads per kv head, pages of 16 .. 1024 "
+                   "positions in powers of two, T in [1, 65536], table positions below 2^31 - 4096)";
         case RV12_E_LAUNCH: return "kernel launch failed";
     }
     return "unknown rv12 status";
@@ -775,6 +778,92 @@ int rv12_prefill_rope_attn(const rv12_attn* a, int t, const float* qkv, const fl
     p.scale = a->scale;
     p.T = t;
     if (launch_prefill_attn(p, (hipStream_t)stream)) return RV12_E_CONFIG;
+    return launch_status();
+}
+
+// --- paged cache
+static int paged_params(const rv12_paged* a, int t, PagedParams* p) {
+    if (!a) return RV12_E_NULL;
+    if (a->head_dim != 64 && a->head_dim != 128) return RV12_E_PAGED;
+    if (a->n_kv < 1 || a->n_kv > 256 || a->n_heads < a->n_kv || a->n_heads % a->n_kv) return RV12_E_PAGED;
+    const int g = a->n_heads / a->n_kv;
+    if (g > 16) return RV12_E_PAGED;
+    if (a->page < 16 || a->page > 1024 || (a->page & (a->page - 1))) return RV12_E_PAGED;
+    if (a->n_seq < 1 || a->max_pages < 1 || a->n_pages < 1 || a->n_pages > 0x7FFFFFFF || a->table_stride < a->max_pages)
+        return RV12_E_PAGED;
+    const int64_t cap = (int64_t)a->max_pages * a->page;
+    if (cap > (int64_t)0x7FFFFFFF - 4096 || t < 1 || t > kMaxPagedRows) return RV12_E_PAGED;
+    p->T = t;
+    p->n_heads = a->n_heads;
+    p->n_kv = a->n_kv;
+    p->head_dim = a->head_dim;
+    p->kv_bf16 = a->kv_bf16 ? 1 : 0;
+    p->page_log = __builtin_ctz((unsigned)a->page);
+    p->n_seq = a->n_seq;
+    p->g = g;
+    p->rt = 1;
+    while (p->rt * 2 * g <= 16) p->rt *= 2;
+    p->table_stride = a->table_stride;
+    p->n_pages = a->n_pages;
+    p->cap = cap;
+    p->eps = a->eps;
+    p->scale = a->scale;
+    // the plan's chunk length stays an int
+    if ((double)t * (double)cap * a->n_kv / p->target > (double)(1 << 30)) return RV12_E_PAGED;
+    return RV12_OK;
+}
+
+int rv12_paged_append(const rv12_paged* a, int t, const float* qkv, const float* qn, const float* kn, const float* inv,
+                      const int32_t* seq, const int64_t* pos, const int32_t* table, void* kc, void* vc, float* q,
+                      void* stream) {
+    PagedParams p;
+    const int rc = paged_params(a, t, &p);
+    if (rc) return rc;
+    if (!qkv || !qn || !kn || !inv || !pos || !table || !kc || !vc || !q) return RV12_E_NULL;
+    if (!aligned16(qkv) || !aligned16(qn) || !aligned16(kn) || !aligned16(kc) || !aligned16(vc) || !aligned16(q) ||
+        ((uintptr_t)pos & 7u) || (((uintptr_t)inv | (uintptr_t)seq | (uintptr_t)table) & 3u))
+        return RV12_E_ALIGN;
+    p.qkv = qkv;
+    p.qn = qn;
+    p.kn = kn;
+    p.inv = inv;
+    p.seq = seq;
+    p.pos = pos;
+    p.table = table;
+    p.kc = kc;
+    p.vc = vc;
+    p.qo = q;
+    launch_paged_append(p, (hipStream_t)stream);
+    return launch_status();
+}
+
+size_t rv12_paged_attend_workspace_bytes(const rv12_paged* a, int t) {
+    PagedParams p;
+    if (paged_params(a, t, &p)) return 0;
+    return 16 + (size_t)paged_slots(p) * p.n_kv * (p.rt * p.g) * (p.head_dim + 2) * 4;
+}
+
+int rv12_paged_attend(const rv12_paged* a, int t, const float* q, const int32_t* seq, const int64_t* pos,
+                      const int32_t* table, const void* kc, const void* vc, float* out, void* ws, size_t ws_bytes,
+                      void* stream) {
+    PagedParams p;
+    const int rc = paged_params(a, t, &p);
+    if (rc) return rc;
+    if (!q || !pos || !table || !kc || !vc || !out) return RV12_E_NULL;
+    if (!aligned16(q) || !aligned16(kc) || !aligned16(vc) || !aligned16(out) || ((uintptr_t)pos & 7u) ||
+        (((uintptr_t)seq | (uintptr_t)table) & 3u))
+        return RV12_E_ALIGN;
+    if (!ws || ws_bytes < rv12_paged_attend_workspace_bytes(a, t)) return RV12_E_WORKSPACE;
+    if (!aligned16(ws)) return RV12_E_ALIGN;
+    p.q = q;
+    p.seq = seq;
+    p.pos = pos;
+    p.table = table;
+    p.kc = const_cast<void*>(kc);
+    p.vc = const_cast<void*>(vc);
+    p.out = out;
+    p.part = (float*)ws;
+    launch_paged_attend(p, (hipStream_t)stream);
     return launch_status();
 }
 

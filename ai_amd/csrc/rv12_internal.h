@@ -4,6 +4,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "rv12.h"
 
 namespace rv12 {
@@ -168,6 +170,43 @@ int launch_attn_batch(const AttnParams& p, int splits, hipStream_t st);
 // float32 matrix cores (one wave per head and 16 tokens)
 constexpr int kMaxPrefillAttnTokens = 1 << 15;  // the prologue grid's second dimension stays below 65536
 int launch_prefill_attn(const AttnParams& p, hipStream_t st);
+
+// --- paged cache: append and attention of T token rows
+struct PagedParams {
+    const float* qkv = nullptr;
+    const float* qn = nullptr;
+    const float* kn = nullptr;
+    const float* inv = nullptr;
+    const int32_t* seq = nullptr;  // NULL: row r is of sequence r
+    const int64_t* pos = nullptr;
+    const int32_t* table = nullptr;
+    void* kc = nullptr;
+    void* vc = nullptr;
+    const float* q = nullptr;
+    float* qo = nullptr;
+    float* out = nullptr;
+    float* part = nullptr;  // [slots][n_kv][rt g][HD + 2] partials of rows in several chunks
+    int T, n_heads, n_kv, head_dim, kv_bf16, page_log, n_seq;
+    int g;   // query heads per kv head
+    int rt;  // rows of one sequence that share a workgroup's 16 columns at most
+    int target = 1024, min_chunk = 128;
+    int64_t table_stride, n_pages, cap;  // cap: positions the table covers
+    float eps, scale;
+};
+constexpr int kMaxPagedRows = 1 << 16;
+// workgroups per kv head at most: every row has a chunk, and rows of n > C
+// positions have fewer than n / C + 1, the sum of n being at most C target / n_kv
+inline int64_t paged_items(const PagedParams& p) {
+    const int64_t c = (p.min_chunk + 127) / 128 * 128;
+    return std::min((int64_t)p.target / p.n_kv + p.T, (int64_t)p.T * ((p.cap + c - 1) / c));
+}
+// rows of several chunks at most (n > C each), and their chunks (fewer than 2 n / C each)
+inline int paged_split_rows(const PagedParams& p) {
+    return p.cap <= (p.min_chunk + 127) / 128 * 128 ? 0 : std::min(p.T, p.target / p.n_kv);
+}
+inline int paged_slots(const PagedParams& p) { return paged_split_rows(p) ? 2 * (p.target / p.n_kv) : 0; }
+void launch_paged_append(const PagedParams& p, hipStream_t st);
+void launch_paged_attend(const PagedParams& p, hipStream_t st);
 
 int launch_gemv(const LinearParams& p, int T, int rb, int waves, int splits, hipStream_t st);
 // ks: the waves of a workgroup split its K steps (kernel 3) instead of its rows (kernel 2)

@@ -36,6 +36,7 @@ enum rv12_status {
     RV12_E_ALIGN = -8,     /* x, y or tiles not 16-byte aligned */
     RV12_E_SIZE = -9,      /* output buffer smaller than rv12_tiles_bytes() */
     RV12_E_SCRATCH = -10,  /* rv12_gemm_static: workspace beyond RV12_STATIC_SCRATCH_BYTES */
+    RV12_E_PAGED = -11,    /* rv12_paged out of range, or t outside [1, 65536] */
     RV12_E_LAUNCH = -20    /* hipGetLastError() after a launch */
 };
 
@@ -349,6 +350,55 @@ size_t rv12_prefill_attn_workspace_bytes(const rv12_attn* a, int t);
 int rv12_prefill_rope_attn(const rv12_attn* a, int t, const float* qkv, const float* qn, const float* kn,
                            const float* inv, const int64_t* pos, void* kc, void* vc, float* out, void* ws,
                            size_t ws_bytes, void* stream);
+
+/* A key-value cache of many sequences in pages.  kc and vc are
+ * [n_pages][n_kv][page][head_dim] (bf16 bits or float32); position j of sequence
+ * s is slot j % page of page table[s * table_stride + j / page] (int32).  A pass
+ * has 1 <= t <= 65536 token rows: row r is position pos[r] (int64) of sequence
+ * seq[r] (int32; seq NULL: sequence r), all read on the device, so a captured
+ * graph can advance them.  A row whose sequence is outside [0, n_seq) or whose
+ * position is outside [0, max_pages page) is padding.  A page id outside
+ * [0, n_pages) is no page.  head_dim 64 or 128; n_heads / n_kv 1 .. 16; page a
+ * power of two, 16 .. 1024; max_pages page below 2^31 - 4096 and t max_pages page
+ * n_kv at most 2^40. */
+typedef struct rv12_paged {
+    int32_t n_heads, n_kv, head_dim, page;
+    int32_t kv_bf16; /* 1: bf16 caches, 0: float32 */
+    int32_t n_seq, max_pages;
+    int64_t table_stride, n_pages;
+    float eps, scale;
+} rv12_paged;
+
+/* The rows' keys and values into their pages: q and k of qkv (t rows of (n_heads +
+ * 2 n_kv) * head_dim floats) get the head RMSNorm (qn, kn: float[head_dim]) and the
+ * rotate-half RoPE at the row's position (angle pos * inv[i], formed in 64 bits:
+ * exact where rv12_rope_attn's float32 product is not, from positions of some
+ * thousands on); q goes to q (t rows of n_heads * head_dim floats), k and v,
+ * rounded once to the cache type, to the row's slot.  A padding row's q is zeros
+ * and nothing is written for it; a row whose page is none writes no key or value.
+ * Two rows of one slot: which of them it then holds is not defined.  qkv, qn, kn,
+ * q, kc, vc 16-byte aligned.  The paged counterpart of qk_rope_cache_k,
+ * ramvi/engine/ramvi_engine/kernels/tkernels.py:82-120. */
+int rv12_paged_append(const rv12_paged* a, int t, const float* qkv, const float* qn, const float* kn, const float* inv,
+                      const int32_t* seq, const int64_t* pos, const int32_t* table, void* kc, void* vc, float* q,
+                      void* stream);
+
+/* The rows' attention: out[r] (t rows of n_heads * head_dim floats) is the
+ * grouped-query attention of q[r] over positions 0 .. pos[r] of its sequence,
+ * softmax(q . K scale) V, float32 products and sums.  The keys and values of those
+ * positions, the rows' own among them, are in the cache before the call.
+ * Positions without a page take no part; a row that is padding, or has nothing
+ * left to attend, gives zeros.  Slots past a row's position are not read into it,
+ * whatever they hold.  Two passes (chunks of positions, about 1024 workgroups
+ * whatever the lengths; the join of the rows in several chunks, in chunk order),
+ * no atomics.  ws: rv12_paged_attend_workspace_bytes(a, t) bytes, 16-byte aligned
+ * (0 bytes there: a or t out of range); calls that overlap need their own.  The
+ * paged counterpart of rope_attn_k's and attn_k's attention,
+ * ramvi/engine/ramvi_engine/kernels/tkernels.py:123-213. */
+size_t rv12_paged_attend_workspace_bytes(const rv12_paged* a, int t);
+int rv12_paged_attend(const rv12_paged* a, int t, const float* q, const int32_t* seq, const int64_t* pos,
+                      const int32_t* table, const void* kc, const void* vc, float* out, void* ws, size_t ws_bytes,
+                      void* stream);
 
 #ifdef __cplusplus
 }

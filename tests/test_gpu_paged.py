@@ -1,0 +1,404 @@
+"""The paged cache (rv12_paged_append, rv12_paged_attend through
+attn.PagedRopeAttn) against the same formulas in float64.
+
+Tolerances, from the kernels' roundings (u = 2^-24):
+  append   q and k after the rotation, per unit of |x| + |y| of the rotated pair:
+           12 roundings of the sum of squares halved by the root, 4 of the root, 2
+           of the products, the reduced angle (2 u) and its sine or cosine (4 u),
+           2 of the rotation: below 20 u; the cache's own rounding on top (half a
+           step, 2^-8 in bf16); v is rounded only
+  attend   a score is a sum of HD products in float32: off by at most (HD + 4) u
+           sum |q k| scale; a weight by twice that (its own and the sum's) and 2^-21
+           for the exponential; the sums over positions run in chains of at most
+           112 steps per 128 positions of a chunk and one per chunk"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+EPS = 1e-6
+HEADS = [(32, 8, 128), (16, 8, 128), (40, 8, 128), (64, 8, 128), (8, 4, 64), (6, 2, 64), (16, 1, 128), (7, 7, 64),
+         (44, 4, 128)]
+KV_TYPES = [torch.float32, torch.bfloat16]
+
+
+def _inv(HD):
+    return (1.0 / (1e6 ** (torch.arange(0, HD, 2, dtype=torch.float32) / HD))).cuda()
+
+
+def _gen(*key):
+    return torch.Generator(device="cuda").manual_seed(hash(key) % (1 << 31))
+
+
+def _randn(g, *shape):
+    return torch.randn(*shape, generator=g, device="cuda")
+
+
+def _table(lens, page, g, extra=2, pad=1):
+    """page ids of every sequence, shuffled over the pool, -1 past its end."""
+    need = [-(-n // page) for n in lens]
+    n_pages = sum(need) + extra
+    ids = torch.randperm(n_pages, generator=g, device="cuda").tolist()
+    t = torch.full((len(lens), max(need + [1]) + pad), -1, dtype=torch.int32)
+    at = 0
+    for i, n in enumerate(need):
+        t[i, :n] = torch.tensor(ids[at:at + n], dtype=torch.int32)
+        at += n
+    return t.cuda(), n_pages
+
+
+def _append_ref(qkv, qn, kn, inv, pos, H, KV, HD):
+    """(q, k, v, bound per unit roundoff of q, of k) in float64 for the rows."""
+    T = len(qkv)
+    x = qkv.double().view(T, H + 2 * KV, HD)
+    ang = pos.double()[:, None] * inv.double()
+    c, s = ang.cos()[:, None], ang.sin()[:, None]
+
+    def rot(h, w):
+        h = h * (h.square().mean(-1, keepdim=True) + EPS).rsqrt() * w.double()
+        a, b = h.chunk(2, -1)
+        return torch.cat([a * c - b * s, b * c + a * s], -1), (a.abs() + b.abs()).repeat(1, 1, 2)
+    q, qb = rot(x[:, :H], qn)
+    k, kb = rot(x[:, H:H + KV], kn)
+    return q, k, x[:, H + KV:], 20 * U * qb, 20 * U * kb
+
+
+@pytest.mark.parametrize("H,KV,HD", HEADS)
+@pytest.mark.parametrize("kv", KV_TYPES)
+@pytest.mark.parametrize("page", [16, 64, 1024])
+def test_append_matches_float64(H, KV, HD, kv, page):
+    from ai_amd.attn import PagedRopeAttn
+    g = _gen(H, KV, HD, page)
+    lens = [1, page, page + 1, 3 * page - 1, 200, 40001]
+    print("case", H, KV, HD, kv, page, flush=True)
+    table, n_pages = _table(lens, page, g)
+    # rows: the last of every sequence, a run of the fifth's, padding of each kind, a page that is none
+    seq = [0, 1, 2, 3, 5] + [4] * 9 + [-1, 6, 2, 1, 3, 5]
+    pos = [0, page - 1, page, 3 * page - 2, 40000] + list(range(150, 159)) + [5, 0, -1, table.shape[1] * page, 2, 17]
+    table[3, 0] = n_pages  # row (3, 2): past the pool; row (5, 17): -1
+    table[5, 17 // page] = -1
+    T = len(seq)
+    seq_t = torch.tensor(seq, dtype=torch.int32, device="cuda")
+    pos_t = torch.tensor(pos, dtype=torch.int64, device="cuda")
+    qkv = _randn(g, T, (H + 2 * KV) * HD) * 2
+    qkv[7] *= 1e4
+    qkv[8] = 0
+    qn, kn = 1 + 0.2 * _randn(g, HD), 1 + 0.2 * _randn(g, HD)
+    inv = _inv(HD)
+    kc, vc = _randn(g, n_pages, KV, page, HD).to(kv), _randn(g, n_pages, KV, page, HD).to(kv)
+    kc0, vc0 = kc.clone(), vc.clone()
+    q = torch.full((T, H * HD), float("nan"), device="cuda")
+    p = PagedRopeAttn(H, KV, HD, page, kv, EPS)
+    p.append(qkv, qn, kn, inv, seq_t, pos_t, table, kc, vc, q)
+    torch.cuda.synchronize()
+    rq, rk, rv, bq, bk = _append_ref(qkv, qn, kn, inv, pos_t, H, KV, HD)
+    live = [r for r in range(T) if 0 <= seq[r] < len(lens) and 0 <= pos[r] < table.shape[1] * page]
+    dead = [r for r in range(T) if r not in live]
+    assert dead == [14, 15, 16, 17] and torch.equal(q[dead], torch.zeros_like(q[dead]))
+    assert bool(((q[live].double().view(-1, H, HD) - rq[live]).abs() <= bq[live]).all())
+    touched = torch.zeros(n_pages, page, dtype=torch.bool, device="cuda")
+    half = torch.finfo(kv).eps / 2
+    for r in live:
+        pid = int(table[seq[r], pos[r] // page])
+        if not 0 <= pid < n_pages:
+            continue
+        at = pos[r] % page
+        touched[pid, at] = True
+        assert bool(((kc[pid, :, at].double() - rk[r]).abs() <= bk[r] + half * (rk[r].abs() + bk[r])).all()), r
+        assert torch.equal(vc[pid, :, at], rv[r].to(kv)), r
+    assert int(touched.sum()) == len(live) - 2
+    keep = ~touched[:, None, :, None].expand_as(kc)
+    assert torch.equal(kc[keep], kc0[keep]) and torch.equal(vc[keep], vc0[keep])
+
+
+def _attend_ref(q, seq, pos, table, kc, vc, H, KV, HD, page):
+    """(out, bound) in float64; None entries of the table take no part."""
+    T, G = len(q), H // KV
+    out = torch.zeros(T, H, HD, dtype=torch.float64, device="cuda")
+    bound = torch.zeros_like(out)
+    scale = HD ** -0.5
+    seq, pos, tab = seq.tolist(), pos.tolist(), table.cpu()
+    cap = table.shape[1] * page
+    for r in range(T):
+        if not (0 <= seq[r] < len(tab) and 0 <= pos[r] < cap):
+            continue
+        n = pos[r] + 1
+        ids = tab[seq[r], :-(-n // page)].long()
+        ok = ((ids >= 0) & (ids < kc.shape[0])).repeat_interleave(page)[:n].cuda()
+        if not bool(ok.any()):
+            continue
+        ids = ids.clamp(0, kc.shape[0] - 1).cuda()
+        K, V = (c[ids].double().transpose(0, 1).reshape(KV, -1, HD)[:, :n][:, ok].contiguous() for c in (kc, vc))
+        qr = q[r].double().view(KV, G, HD)
+        Kt = K.transpose(1, 2).contiguous()
+        s = torch.matmul(qr, Kt) * scale
+        a = torch.softmax(s, -1)
+        out[r] = torch.matmul(a, V).reshape(H, HD)
+        delta = (HD + 4) * U * (torch.matmul(qr.abs(), Kt.abs()) * scale).amax(-1, keepdim=True)
+        rel = 4 * delta + 2.0 ** -21 + (112 * max(1, n / 128) + 64) * U
+        bound[r] = (rel * torch.matmul(a, V.abs())).reshape(H, HD)
+    return out, bound
+
+
+def _check(p, q, seq, pos, table, kc, vc, what=""):
+    out = torch.full_like(q, float("nan"))
+    s = torch.arange(len(q), device="cuda") if seq is None else seq
+    p.attend(q, seq, pos, table, kc, vc, out)
+    torch.cuda.synchronize()
+    ref, bound = _attend_ref(q, s, pos, table, kc, vc, p.n_heads, p.n_kv, p.head_dim, p.page)
+    err = (out.double().view_as(ref) - ref).abs()
+    assert bool((err <= bound).all()), (what, float((err - bound).max()), float((err / bound.clamp(min=1e-300)).max()))
+    return out
+
+
+@pytest.mark.parametrize("H,KV,HD", HEADS)
+@pytest.mark.parametrize("kv", KV_TYPES)
+@pytest.mark.parametrize("page", [16, 128])
+def test_attend_new_tokens(H, KV, HD, kv, page):
+    """One row per sequence, lengths at the edges of blocks, pages and chunks;
+    the slots past each sequence's end hold NaN and infinities."""
+    from ai_amd.attn import PagedRopeAttn
+    g = _gen(H, KV, HD, page, 1)
+    lens = [1, 2, 15, 16, 17, 31, 32, 33, 127, 128, 129, 255, 257, 1000, 2049]
+    print("case", H, KV, HD, kv, page, flush=True)
+    table, n_pages = _table(lens, page, g)
+    kc, vc = _randn(g, n_pages, KV, page, HD).to(kv), _randn(g, n_pages, KV, page, HD).to(kv)
+    used = torch.zeros(n_pages, page, dtype=torch.bool, device="cuda")
+    for i, n in enumerate(lens):
+        for j in range(-(-n // page)):
+            used[int(table[i, j]), :min(page, n - j * page)] = True
+    bad = ~used[:, None, :, None].expand_as(kc)
+    kc[bad], vc[bad] = float("nan"), float("inf")
+    q = _randn(g, len(lens), H * HD) * 2
+    pos = torch.tensor([n - 1 for n in lens], device="cuda")
+    p = PagedRopeAttn(H, KV, HD, page, kv, EPS)
+    a = _check(p, q, None, pos, table, kc, vc)
+    # the same rows through seq, in another order with padding between them
+    order = torch.randperm(len(lens), generator=g, device="cuda")
+    seq = torch.cat([order[:4], torch.tensor([-1, 99], device="cuda"), order[4:]]).int()
+    at = seq.clamp(0, len(lens) - 1).long()
+    b = _check(p, q[at].contiguous(), seq, pos[at].contiguous(), table, kc, vc)
+    assert torch.equal(b[[0, 1, 2, 3]], a[order[:4]]) and not bool(b[[4, 5]].any())
+    # one sequence alone, many chunks of it
+    for i in (0, 8, 14):
+        _check(p, q[i:i + 1].contiguous(), torch.tensor([i], dtype=torch.int32, device="cuda"), pos[i:i + 1].contiguous(),
+               table, kc, vc, i)
+
+
+@pytest.mark.parametrize("H,KV,HD", HEADS)
+@pytest.mark.parametrize("kv", KV_TYPES)
+def test_attend_rows_of_one_sequence(H, KV, HD, kv):
+    """Chunks of a prompt and speculated tokens: every row sees its own past
+    only, whatever the rows beside it; also out of order and repeated."""
+    from ai_amd.attn import PagedRopeAttn
+    page = 32
+    g = _gen(H, KV, HD, 2)
+    lens = [5, 16, 77, 300]
+    print("case", H, KV, HD, kv, flush=True)
+    table, n_pages = _table(lens, page, g)
+    kc, vc = _randn(g, n_pages, KV, page, HD).to(kv), _randn(g, n_pages, KV, page, HD).to(kv)
+    rows = [(0, j) for j in range(5)] + [(1, j) for j in range(16)] + [(2, j) for j in range(60, 77)] + \
+        [(3, j) for j in range(290, 300)] + [(3, 10), (3, 9), (3, 9), (-1, 0), (0, 4), (0, -1), (0, 2), (3, 299)]
+    seq = torch.tensor([r[0] for r in rows], dtype=torch.int32, device="cuda")
+    pos = torch.tensor([r[1] for r in rows], device="cuda")
+    q = _randn(g, len(rows), H * HD) * 2
+    p = PagedRopeAttn(H, KV, HD, page, kv, EPS)
+    out = _check(p, q, seq, pos, table, kc, vc)
+    again = torch.empty_like(out)
+    p.attend(q, seq, pos, table, kc, vc, again)
+    assert torch.equal(out, again)
+    # the last position of sequence 0 holds NaN and infinity: its own rows alone have them
+    last = int(table[0, 0])
+    kc[last, :, 4], vc[last, :, 4] = float("nan"), float("inf")
+    o2 = torch.empty_like(out)
+    p.attend(q, seq, pos, table, kc, vc, o2)
+    hit = (seq == 0) & (pos == 4)
+    assert bool(o2[hit].isnan().all()) and torch.equal(o2[~hit], out[~hit])
+
+
+@pytest.mark.parametrize("kv", KV_TYPES)
+def test_attend_missing_pages(kv):
+    """Pages given back (-1) or out of range take no part; a row left with
+    nothing, and rows of scores all -inf, give zeros."""
+    from ai_amd.attn import PagedRopeAttn
+    H, KV, HD, page = 32, 8, 128, 16
+    g = _gen(3)
+    lens = [600, 600, 40, 16, 20]
+    table, n_pages = _table(lens, page, g)
+    table[0, 3:30] = -1
+    table[0, 35] = n_pages
+    table[1, :] = -1          # nothing left
+    table[2, 2] = -7          # the last page
+    table[4, 0] = 0x7FFFFFFF  # its own page alone is left
+    kc, vc = _randn(g, n_pages, KV, page, HD).to(kv), _randn(g, n_pages, KV, page, HD).to(kv)
+    pos = torch.tensor([n - 1 for n in lens], device="cuda")
+    q = _randn(g, len(lens), H * HD) * 2
+    p = PagedRopeAttn(H, KV, HD, page, kv, EPS)
+    out = _check(p, q, None, pos, table, kc, vc)
+    assert not bool(out[1].any())
+    # scores of -inf: a key of -inf against a positive query
+    q[3] = 1.0
+    kc[int(table[3, 0])] = -float("inf")
+    p.attend(q, None, pos, table, kc, vc, out)
+    torch.cuda.synchronize()
+    ref, bound = _attend_ref(q[:3], torch.arange(3), pos[:3], table, kc, vc, H, KV, HD, page)
+    assert bool(((out[:3].double().view_as(ref) - ref).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("kv", KV_TYPES)
+def test_long_contexts_and_many_rows(kv):
+    """A 30000-position sequence in many chunks beside short ones, more than 64
+    rows (several steps of the plan), and rows of one sequence over its end."""
+    from ai_amd.attn import PagedRopeAttn
+    H, KV, HD, page = 32, 8, 128, 64
+    g = _gen(4)
+    lens = [30000] + [3 + 7 * i for i in range(90)] + [5000]
+    table, n_pages = _table(lens, page, g)
+    kc, vc = _randn(g, n_pages, KV, page, HD).to(kv), _randn(g, n_pages, KV, page, HD).to(kv)
+    rows = [(i, n - 1) for i, n in enumerate(lens[:-1])] + [(len(lens) - 1, 5000 - 11 + j) for j in range(11)]
+    seq = torch.tensor([r[0] for r in rows], dtype=torch.int32, device="cuda")
+    pos = torch.tensor([r[1] for r in rows], device="cuda")
+    q = _randn(g, len(rows), H * HD)
+    p = PagedRopeAttn(H, KV, HD, page, kv, EPS)
+    _check(p, q, seq, pos, table, kc, vc)
+
+
+def test_offsets_past_32_bits():
+    """Caches of more than 2^32 bytes and 2^31 values: pages at their end."""
+    from ai_amd.attn import PagedRopeAttn
+    H, KV, HD, page = 16, 8, 128, 64
+    n_pages = (1 << 31) // (KV * page * HD) + 40000 // page + 8  # 2^31 values and some more, each bf16
+    kc = torch.empty(n_pages, KV, page, HD, dtype=torch.bfloat16, device="cuda")
+    vc = torch.empty_like(kc)
+    g = _gen(5)
+    m = 500 // page + 1
+    kc[-m:], vc[-m:] = _randn(g, m, KV, page, HD).bfloat16(), _randn(g, m, KV, page, HD).bfloat16()
+    table = torch.arange(n_pages - 1, n_pages - m - 1, -1, dtype=torch.int32, device="cuda")[None].contiguous()
+    p = PagedRopeAttn(H, KV, HD, page, torch.bfloat16, EPS)
+    pos = torch.tensor([499], device="cuda")
+    qkv = _randn(g, 1, (H + 2 * KV) * HD)
+    ones = torch.ones(HD, device="cuda")
+    q = torch.empty(1, H * HD, device="cuda")
+    p.append(qkv, ones, ones, _inv(HD), None, pos, table, kc, vc, q)
+    torch.cuda.synchronize()
+    pid = int(table[0, 499 // page])
+    assert torch.equal(vc[pid, :, 499 % page], qkv.view(-1, HD)[H + KV:].bfloat16())
+    _check(p, q, None, pos, table, kc, vc)
+
+
+def test_against_the_contiguous_cache():
+    """A short decode through pages and through RopeAttn's contiguous cache: the
+    same outputs within both kernels' bounds."""
+    from ai_amd.attn import PagedRopeAttn, RopeAttn
+    H, KV, HD, page, n = 16, 8, 128, 16, 70
+    g = _gen(6)
+    inv, qn, kn = _inv(HD), 1 + 0.1 * _randn(g, HD), 1 + 0.1 * _randn(g, HD)
+    kc, vc = (torch.zeros(KV, 128, HD, device="cuda") for _ in range(2))
+    table, n_pages = _table([n, n], page, g)
+    pk, pv = (torch.zeros(n_pages, KV, page, HD, device="cuda") for _ in range(2))
+    a = RopeAttn(H, KV, HD, 128, torch.float32, EPS, "cuda")
+    p = PagedRopeAttn(H, KV, HD, page, torch.float32, EPS)
+    o1, o2 = torch.empty(H * HD, device="cuda"), torch.empty(2, H * HD, device="cuda")
+    for i in range(n):
+        qkv = _randn(g, (H + 2 * KV) * HD)
+        pos = torch.tensor([i, i], device="cuda")
+        a(qkv, qn, kn, inv, pos[:1], kc, vc, o1)
+        p(torch.stack([qkv, qkv]), qn, kn, inv, None, pos, table, pk, pv, o2)
+        # positions below 70: the float32 angle is off by 70 u at most
+        assert torch.equal(o2[0], o2[1])
+        assert torch.allclose(o2[0], o1, rtol=1e-4, atol=2e-5), i
+
+
+@pytest.mark.parametrize("kv", KV_TYPES)
+def test_graph_replays_follow_the_device(kv):
+    """One captured step replayed with other positions, pages and sequences,
+    with eager calls of the same object between the replays on another stream."""
+    from ai_amd.attn import PagedRopeAttn
+    H, KV, HD, page = 32, 8, 128, 16
+    g = _gen(7)
+    lens = [900, 40, 333]
+    table, n_pages = _table(lens, page, g)
+    inv, qn, kn = _inv(HD), 1 + 0.1 * _randn(g, HD), 1 + 0.1 * _randn(g, HD)
+    kc, vc = _randn(g, n_pages, KV, page, HD).to(kv), _randn(g, n_pages, KV, page, HD).to(kv)
+    T = 4
+    p = PagedRopeAttn(H, KV, HD, page, kv, EPS)
+    qkv, out = torch.zeros(T, (H + 2 * KV) * HD, device="cuda"), torch.zeros(T, H * HD, device="cuda")
+    seq, pos = torch.zeros(T, dtype=torch.int32, device="cuda"), torch.zeros(T, dtype=torch.int64, device="cuda")
+    tab = table.clone()
+    args = (qn, kn, inv, seq, pos, tab)
+    p(qkv, *args, kc.clone(), vc.clone(), out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    gk, gv = kc.clone(), vc.clone()
+    with torch.cuda.graph(graph):
+        p(qkv, *args, gk, gv, out)
+    ek, ev, eo = kc.clone(), vc.clone(), torch.zeros_like(out)
+    for k in range(4):
+        qkv.copy_(_randn(g, *qkv.shape))
+        seq.copy_(torch.tensor([[0, 1, 2, -1], [2, 2, 2, 0], [1, -1, 0, 0], [0, 0, 0, 0]][k]))
+        pos.copy_(torch.tensor([[800, 39, 0, 0], [300, 301, 302, 17], [0, 5, 899, 898], [1, 2, 3, 4]][k]))
+        if k == 2:
+            tab.copy_(table.flip(0))
+            tab[0, 0], tab[1, 0], tab[2, 0] = table[2, 0], table[1, 0], table[0, 0]
+        torch.cuda.synchronize()
+        graph.replay()
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            p(qkv, *args, ek, ev, eo)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eo) and torch.equal(gk, ek) and torch.equal(gv, ev), k
+
+
+def test_table_strides_and_empty_pass():
+    from ai_amd.attn import PagedRopeAttn
+    H, KV, HD, page = 8, 4, 64, 16
+    g = _gen(8)
+    table, n_pages = _table([100, 37], page, g)
+    wide = torch.full((2, 50), -1, dtype=torch.int32, device="cuda")
+    wide[:, 3:3 + table.shape[1]] = table
+    view = wide[:, 3:3 + table.shape[1]]
+    kc, vc = _randn(g, n_pages, KV, page, HD), _randn(g, n_pages, KV, page, HD)
+    p = PagedRopeAttn(H, KV, HD, page, torch.float32, EPS)
+    q = _randn(g, 2, H * HD)
+    pos = torch.tensor([99, 36], device="cuda")
+    assert torch.equal(_check(p, q, None, pos, view, kc, vc), _check(p, q, None, pos, table, kc, vc))
+    p.attend(q[:0], None, pos[:0], table, kc, vc, torch.empty(0, H * HD, device="cuda"))
+    # another scale
+    p2 = PagedRopeAttn(H, KV, HD, page, torch.float32, EPS, scale=0.0)
+    out = torch.empty_like(q)
+    p2.attend(q, None, pos, table, kc, vc, out)
+    mean = vc[table[0, :7].long()].double().transpose(0, 1).reshape(KV, -1, HD)[:, :100].mean(1)
+    assert torch.allclose(out[0].view(KV, 2, HD).double(), mean[:, None].expand(-1, 2, -1), rtol=0, atol=1e-5)
+
+
+def test_refusals():
+    from ai_amd.attn import PagedRopeAttn
+    H, KV, HD, page = 8, 4, 64, 16
+    p = PagedRopeAttn(H, KV, HD, page, torch.float32, EPS)
+    kc = torch.zeros(3, KV, page, HD, device="cuda")
+    table = torch.zeros(2, 2, dtype=torch.int32, device="cuda")
+    q, out = torch.zeros(2, H * HD, device="cuda"), torch.zeros(2, H * HD, device="cuda")
+    pos, seq = torch.zeros(2, dtype=torch.int64, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    good = dict(q=q, seq=seq, pos=pos, table=table, kc=kc, vc=kc.clone(), out=out)
+    p.attend(**good)
+    big = torch.zeros(2, 2 * H * HD, device="cuda")
+    for bad in (dict(q=q.double()), dict(q=big[:, ::2]), dict(q=q[:1]), dict(q=q.cpu()), dict(pos=pos.int()),
+                dict(pos=pos[:1]), dict(seq=seq.long()), dict(seq=seq[:1]), dict(seq=seq.cpu()), dict(table=table.long()),
+                dict(table=table[0]), dict(table=table.t()[:, :1].t().t()[:0]), dict(table=table.cpu()),
+                dict(kc=kc.bfloat16()), dict(vc=kc[:2]), dict(kc=kc.transpose(0, 1)), dict(kc=kc[..., :32]),
+                dict(table=table[:1].expand(2, 2)), dict(out=out[:, :-1])):
+        with pytest.raises(ValueError):
+            p.attend(**{**good, **bad})
+    a = dict(qkv=torch.zeros(2, (H + 2 * KV) * HD, device="cuda"), qn=torch.ones(HD, device="cuda"),
+             kn=torch.ones(HD, device="cuda"), inv=_inv(HD), seq=seq, pos=pos, table=table, kc=kc, vc=kc.clone(), q=q)
+    p.append(**a)
+    off = torch.ones(HD + 1, device="cuda")[1:]
+    for bad in (dict(qkv=a["qkv"][:, :-1]), dict(qn=a["qn"].bfloat16()), dict(kn=a["kn"][:-1]), dict(inv=a["inv"].cpu()),
+                dict(qn=off), dict(q=q.half())):
+        with pytest.raises(ValueError):
+            p.append(**{**a, **bad})
+    torch.cuda.synchronize()
