@@ -18,7 +18,7 @@ LIB_PATH = os.path.join(HERE, "librv12.so")
 RV12_OK = 0
 RV12_E_NULL, RV12_E_SHAPE, RV12_E_MODE, RV12_E_TOKENS = -1, -2, -3, -4
 RV12_E_WORKSPACE, RV12_E_CONFIG, RV12_E_BASE, RV12_E_ALIGN, RV12_E_SIZE, RV12_E_SCRATCH = -5, -6, -7, -8, -9, -10
-RV12_E_PAGED = -11
+RV12_E_PAGED, RV12_E_RULES, RV12_E_LORA = -11, -12, -13
 RV12_E_LAUNCH = -20
 
 # every symbol include/rv12.h declares
@@ -31,7 +31,8 @@ EXPORTS = ("rv12_abi_version", "rv12_strerror", "rv12_tiles_bytes", "rv12_pack_p
            "rv12_prefill_linear", "rv12_decode_advance",
            "rv12_compress_workspace_bytes", "rv12_compress_plan", "rv12_compress_write",
            "rv12_prefill_parts_workspace_bytes", "rv12_prefill_linear_parts",
-           "rv12_paged_append", "rv12_paged_attend_workspace_bytes", "rv12_paged_attend")
+           "rv12_paged_append", "rv12_paged_attend_workspace_bytes", "rv12_paged_attend",
+           "rv12_logits_workspace_bytes", "rv12_logits_adjust", "rv12_lora_workspace_bytes", "rv12_lora_apply")
 ABI_VERSION = 8
 STATIC_SCRATCH_BYTES = 8 << 20  # RV12_STATIC_SCRATCH_BYTES
 
@@ -68,6 +69,17 @@ class Paged(ctypes.Structure):
                 ("page", ctypes.c_int32), ("kv_bf16", ctypes.c_int32), ("n_seq", ctypes.c_int32),
                 ("max_pages", ctypes.c_int32), ("table_stride", ctypes.c_int64), ("n_pages", ctypes.c_int64),
                 ("eps", ctypes.c_float), ("scale", ctypes.c_float)]
+
+
+class Rules(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("tokens", "length", "prompt", "penalties", "bias_ids", "bias", "mask")] + \
+               [(n, ctypes.c_int64) for n in ("tokens_stride", "bias_stride", "mask_stride")] + \
+               [("max_tokens", ctypes.c_int32), ("n_bias", ctypes.c_int32)]
+
+
+class Lora(ctypes.Structure):
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("ranks", ctypes.c_void_p),
+                ("n", ctypes.c_int32), ("k", ctypes.c_int32), ("r", ctypes.c_int32), ("count", ctypes.c_int32)]
 
 
 class Rv12Error(RuntimeError):
@@ -160,6 +172,14 @@ def lib():
         L.rv12_paged_attend_workspace_bytes.argtypes = [ctypes.POINTER(Paged), I]
         L.rv12_paged_attend.restype = I
         L.rv12_paged_attend.argtypes = [ctypes.POINTER(Paged), I, P, P, P, P, P, P, P, P, SZ, P]
+        L.rv12_logits_workspace_bytes.restype = SZ
+        L.rv12_logits_workspace_bytes.argtypes = [I64, I]
+        L.rv12_logits_adjust.restype = I
+        L.rv12_logits_adjust.argtypes = [ctypes.POINTER(Rules), P, I64, P, I64, I64, I, P, P, SZ, P]
+        L.rv12_lora_workspace_bytes.restype = SZ
+        L.rv12_lora_workspace_bytes.argtypes = [I, I, I]
+        L.rv12_lora_apply.restype = I
+        L.rv12_lora_apply.argtypes = [ctypes.POINTER(Lora), P, P, I64, P, I64, P, I, P, F, I, P, SZ, P]
         v = L.rv12_abi_version()
         if v != ABI_VERSION:
             raise RuntimeError(f"librv12.so ABI version {v}, expected {ABI_VERSION}")

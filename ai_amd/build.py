@@ -19,7 +19,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "librv12.so")
 SOURCES = ["rv12_codec.hip", "rv12_gemv.hip", "rv12_gemm.hip", "rv12_prefill.hip", "rv12_attn.hip",
-           "rv12_paged.hip", "rv12_static.hip", "rv12_api.cpp"]
+           "rv12_paged.hip", "rv12_logits.hip", "rv12_lora.hip", "rv12_static.hip", "rv12_api.cpp"]
 HEADERS = ["rv12_device.h", "rv12_internal.h"]
 MANIFEST = OUT + ".build.json"
 PROBE_OUT = os.path.join(HERE, "librv12probe.so")  # bench.py's stream-ceiling probe (not the product)

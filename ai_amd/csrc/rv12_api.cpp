@@ -382,6 +382,9 @@ const char* rv12_strerror(int s) {
         case RV12_E_PAGED:
             return "bad paged cache or rows (head_dim 64 or 128, up to 16 query heads per kv head, pages of 16 .. 1024 "
                    "positions in powers of two, T in [1, 65536], table positions below 2^31 - 4096)";
+        case RV12_E_RULES: return "bad logits or rules (T in [1, 65535], V in [1, 2^31 - 65536), counts and strides >= 0)";
+        case RV12_E_LORA:
+            return "bad adapters (N >= 1, K % 32 == 0, rank a multiple of 8 up to 128, count >= 1) or T outside [1, 65536]";
         case RV12_E_LAUNCH: return "kernel launch failed";
     }
     return "unknown rv12 status";
@@ -864,6 +867,104 @@ int rv12_paged_attend(const rv12_paged* a, int t, const float* q, const int32_t*
     p.out = out;
     p.part = (float*)ws;
     launch_paged_attend(p, (hipStream_t)stream);
+    return launch_status();
+}
+
+// --- rules on logits
+size_t rv12_logits_workspace_bytes(int64_t v, int t) {
+    if (t < 1 || t > 65535 || v < 1 || v >= (int64_t)0x7FFFFFFF - 65535) return 0;
+    return (size_t)adjust_slices(v, t) * t * 8;
+}
+
+int rv12_logits_adjust(const rv12_rules* rules, const float* x, int64_t x_stride, float* y, int64_t y_stride, int64_t v,
+                       int t, int64_t* ids, void* ws, size_t ws_bytes, void* stream) {
+    if (!rules || !x || !y) return RV12_E_NULL;
+    const rv12_rules& a = *rules;
+    if (!rv12_logits_workspace_bytes(v, t)) return RV12_E_RULES;
+    if (a.max_tokens < 0 || a.n_bias < 0 || a.tokens_stride < 0 || a.bias_stride < 0 || a.mask_stride < 0 ||
+        x_stride < 0 || (t > 1 && y_stride < v))
+        return RV12_E_RULES;
+    if (a.tokens && (!a.length || !a.penalties)) return RV12_E_NULL;
+    if (a.n_bias && (!a.bias_ids || !a.bias)) return RV12_E_NULL;
+    if (((uintptr_t)a.tokens | (uintptr_t)a.bias_ids | (uintptr_t)ids) & 7u) return RV12_E_ALIGN;
+    if (((uintptr_t)x | (uintptr_t)y | (uintptr_t)a.length | (uintptr_t)a.prompt | (uintptr_t)a.penalties |
+         (uintptr_t)a.bias | (uintptr_t)a.mask) & 3u)
+        return RV12_E_ALIGN;
+    if (ids && (!ws || ws_bytes < rv12_logits_workspace_bytes(v, t))) return RV12_E_WORKSPACE;
+    if (ids && ((uintptr_t)ws & 7u)) return RV12_E_ALIGN;
+    AdjustParams p;
+    p.x = x;
+    p.y = y;
+    p.V = v;
+    p.x_stride = x_stride;
+    p.y_stride = y_stride;
+    p.tokens = a.tokens;
+    p.tokens_stride = a.tokens_stride;
+    p.length = a.length;
+    p.prompt = a.prompt;
+    p.penalties = a.tokens ? a.penalties : nullptr;
+    p.bias_ids = a.bias_ids;
+    p.bias = a.bias;
+    p.bias_stride = a.bias_stride;
+    p.mask = a.mask;
+    p.mask_stride = a.mask_stride;
+    p.max_tokens = a.max_tokens;
+    p.n_bias = a.n_bias;
+    p.slice = adjust_slice(v, t);
+    if (ids) {
+        p.pv = (float*)ws;
+        p.pi = (int32_t*)ws + adjust_slices(v, t) * t;
+    }
+    launch_adjust(p, t, ids, (hipStream_t)stream);
+    return launch_status();
+}
+
+// --- low-rank adapters
+size_t rv12_lora_workspace_bytes(int r, int k, int t) {
+    if (r < 8 || r % 8 || r > kMaxLoraRank || k < 32 || k % 32 || k > kMaxK || t < 1 || t > 65536) return 0;
+    return (size_t)lora_splits(k, t) * t * (16 * (size_t)lora_rank_blocks(r) + 1) * 4;
+}
+
+int rv12_lora_apply(const rv12_lora* a, const float* x, const float* y, int64_t y_stride, float* out, int64_t out_stride,
+                    const int32_t* idx, int t, const uint16_t* lnw, float eps, int mode, void* ws, size_t ws_bytes,
+                    void* stream) {
+    if (!a) return RV12_E_NULL;
+    const size_t need = rv12_lora_workspace_bytes(a->r, a->k, t);
+    if (!need || a->n < 1 || a->n > 0x7FFFFFFF - 1024 || a->count < 1) return RV12_E_LORA;
+    if (t > 1 && (y_stride < a->n || out_stride < a->n || (y == out && y_stride != out_stride))) return RV12_E_LORA;
+    if (mode < 0 || mode > 2 || (lnw && mode == 2)) return RV12_E_MODE;
+    if (!a->a || !a->b || !a->scale || !x || !y || !out || !idx) return RV12_E_NULL;
+    if (!aligned16(a->a) || !aligned16(a->b) || !aligned16(x) || (lnw && !aligned16(lnw)) ||
+        (((uintptr_t)y | (uintptr_t)out | (uintptr_t)idx | (uintptr_t)a->scale | (uintptr_t)a->ranks) & 3u))
+        return RV12_E_ALIGN;
+    if (!ws || ws_bytes < need) return RV12_E_WORKSPACE;
+    if (!aligned16(ws)) return RV12_E_ALIGN;
+    LoraParams p;
+    p.x = x;
+    p.y = y;
+    p.out = out;
+    p.idx = idx;
+    p.A = a->a;
+    p.B = a->b;
+    p.scale = a->scale;
+    p.ranks = a->ranks;
+    p.lnw = lnw;
+    p.y_stride = y_stride;
+    p.out_stride = out_stride;
+    p.T = t;
+    p.N = a->n;
+    p.K = a->k;
+    p.R = a->r;
+    p.count = a->count;
+    p.mode = mode;
+    p.S = lora_splits(a->k, t);
+    p.slots = t <= 64 ? std::min(t, 16) : 2;
+    p.nbw = 4;
+    p.eps = eps;
+    p.h = (float*)ws;
+    p.ssq = p.h + (size_t)p.S * t * 16 * lora_rank_blocks(a->r);
+    const bool vec = aligned16(y) && aligned16(out) && a->n % 4 == 0 && (t == 1 || (y_stride % 4 == 0 && out_stride % 4 == 0));
+    launch_lora(p, vec, (hipStream_t)stream);
     return launch_status();
 }
 

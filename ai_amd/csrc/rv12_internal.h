@@ -208,6 +208,64 @@ inline int paged_slots(const PagedParams& p) { return paged_split_rows(p) ? 2 * 
 void launch_paged_append(const PagedParams& p, hipStream_t st);
 void launch_paged_attend(const PagedParams& p, hipStream_t st);
 
+// --- rules on logits (k_adjust)
+constexpr int kAdjustThreads = 256;
+struct AdjustParams {
+    const float* x;
+    float* y;
+    int64_t V, x_stride, y_stride;
+    const int64_t* tokens;
+    int64_t tokens_stride;
+    const int32_t* length;
+    const int32_t* prompt;
+    const float* penalties;
+    const int64_t* bias_ids;
+    const float* bias;
+    int64_t bias_stride, mask_stride;
+    const uint32_t* mask;
+    float* pv = nullptr;  // per row and slice the largest allowed value and its id
+    int32_t* pi = nullptr;
+    int max_tokens, n_bias, slice;
+};
+// ids of one workgroup's slice: 4096, less while the rows are too few to fill the GPU
+inline int adjust_slice(int64_t V, int T) {
+    int s = 4096;
+    while (s > 1024 && (V + s - 1) / s * T < 512) s /= 2;
+    return s;
+}
+inline int64_t adjust_slices(int64_t V, int T) { return (V + adjust_slice(V, T) - 1) / adjust_slice(V, T); }
+void launch_adjust(const AdjustParams& p, int T, int64_t* ids, hipStream_t st);
+
+// --- low-rank adapters (k_lora_down, k_lora_up)
+struct LoraParams {
+    const float* x;
+    const float* y;
+    float* out;
+    const int32_t* idx;
+    const uint16_t* A;
+    const uint16_t* B;
+    const float* scale;
+    const int32_t* ranks;
+    const uint16_t* lnw;
+    float* h;    // [S][T][16 rank blocks]
+    float* ssq;  // [S][T]
+    int64_t y_stride, out_stride;
+    int T, N, K, R, count, mode;
+    int S;      // K splits of the first pass
+    int slots;  // adapters of a tile side by side
+    int nbw;    // blocks of 16 output rows per wave of the second pass
+    float eps;
+};
+constexpr int kMaxLoraRank = 128;
+// blocks of 16 ranks the kernels are built for: 1, 2, 4 or 8
+inline int lora_rank_blocks(int R) { return R <= 16 ? 1 : (R <= 32 ? 2 : (R <= 64 ? 4 : 8)); }
+// K splits: 4 steps of 32 columns per wave while the tiles are few
+inline int lora_splits(int K, int T) {
+    const int tiles = (T + 15) / 16, steps = K / 32;
+    return std::max(1, std::min((steps + 15) / 16, 512 / tiles));
+}
+void launch_lora(const LoraParams& p, bool vec, hipStream_t st);
+
 int launch_gemv(const LinearParams& p, int T, int rb, int waves, int splits, hipStream_t st);
 // ks: the waves of a workgroup split its K steps (kernel 3) instead of its rows (kernel 2)
 int launch_gemm(const LinearParams& p, int T, int rbw, int waves, int splits, bool ks, hipStream_t st);

@@ -9,9 +9,7 @@
 // A workgroup takes a slice of one row's vocabulary.  It counts the row's tokens
 // that fall into the slice in LDS (integer adds and maxima: the order does not
 // matter), then passes over the slice once.  The history is read again by every
-// slice, 8 bytes a token from the L2, against 8 bytes per id from HBM: with 8192
-// ids a slice, a history of 8192 tokens doubles the bytes a workgroup reads, all
-// but the first time from the cache.
+// slice, 8 bytes a token from the L2, against 8 bytes per id from HBM.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

@@ -3,7 +3,7 @@
 
     Head(Wu16, TM=16)                          head.py:29-47
     bounds(h, T)                               head.py:49-54 (no bounds are needed here)
-    pick(h, T, temperature, top_p, rng, run_bounds)   head.py:56-88
+    pick(h, T, temperature, top_p, rng, run_bounds, rules)   head.py:56-88 (rules: ai_amd.logits.adjust)
 
 The reference keeps an int8 copy of the vocabulary on the GPU for logit
 bounds and computes the exact fp32 logits of the candidate rows on the CPU
@@ -18,6 +18,7 @@ import numpy as np
 import torch
 
 from . import wcomp
+from .logits import adjust
 
 
 class Head:
@@ -39,20 +40,31 @@ class Head:
         logit is computed exactly; kept so that callers run unchanged."""
         return None
 
-    def pick(self, h, T, temperature=0.0, top_p=1.0, rng=None, run_bounds=True):
+    def pick(self, h, T, temperature=0.0, top_p=1.0, rng=None, run_bounds=True, rules=None):
         """Ids for the T rows of h ([T, D] fp32 on the GPU); temperature 0
-        picks the most likely id, the smallest on ties."""
+        picks the most likely id, the smallest on ties.  rules: the keyword
+        arguments of ai_amd.logits.adjust (tokens, length, prompt, penalties,
+        bias_ids, bias, mask), applied to the logits before the pick; a row
+        whose mask allows no id gets -1."""
         T = int(T)
         x = h[:T].float().contiguous()
-        if temperature <= 0:
+        if temperature <= 0 and not rules:
             wcomp.greedy(x, self.c, T, self.ids)
             return self.ids[:T].tolist()
         if self.logits is None or self.logits.shape[0] < T:
             self.logits = torch.empty(max(T, 1), self.V, device=x.device)
         wcomp.greedy(x, self.c, T, self.ids, logits=self.logits)
+        if rules:
+            adjust(self.logits[:T], ids=self.ids[:T], **rules)
+            if temperature <= 0:
+                return self.ids[:T].tolist()
+            none = self.ids[:T].cpu().numpy() < 0
         lg = self.logits[:T].cpu().numpy().astype(np.float64)
         out = []
         for t in range(T):
+            if rules and none[t]:
+                out.append(-1)
+                continue
             z = (lg[t] - lg[t].max()) / temperature
             p = np.exp(z)
             p /= p.sum()

@@ -1,0 +1,92 @@
+"""Rules on logits before the pick, for many requests at once (rv12_logits_adjust):
+penalties for repeated tokens, biases, grammar masks, and the greedy pick of
+what they leave.  Head.pick applies them between the head and the pick."""
+import ctypes
+
+import torch
+
+from ._lib import Rules, check, lib
+from .wcomp import _ptr, _stream
+
+
+def _rows(t, name, dtype, T, n, dev):
+    """[T, n] (n None: any) with contiguous rows, any stride between them."""
+    if not torch.is_tensor(t) or t.dtype != dtype or t.dim() != 2 or t.device != dev:
+        raise ValueError(f"adjust: {name} must be a 2-D {dtype} tensor on the device of x")
+    if t.shape[0] != T or (n is not None and t.shape[1] != n) or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"adjust: {name} must have {T} rows" + ("" if n is None else f" of {n}") + ", contiguous each")
+    return t.stride(0) if T > 1 else t.shape[1]
+
+
+def _vector(t, name, dtype, T, dev):
+    if not torch.is_tensor(t) or t.dtype != dtype or tuple(t.shape) != (T,) or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"adjust: {name} must be a contiguous {dtype} vector of {T} entries on the device of x")
+
+
+def adjust(x, out=None, tokens=None, length=None, prompt=None, penalties=None, bias_ids=None, bias=None, mask=None,
+           ids=None):
+    """The rules on the logits x (float32 [T, V]) into out (None: in place), which
+    is returned.  Per row and id n, in float32 and this order:
+
+        n among the row's tokens:            l = l / repetition if l > 0 else l * repetition
+        n generated c > 0 times:             l -= frequency * c + presence
+        n in bias_ids:                       l += its bias
+        n not allowed:                       l = -inf, whatever it was
+
+    tokens     int64 [T, L] with length (int32 [T]): row r's tokens are the first
+               length[r]; prompt (int32 [T]): the first prompt[r] of them are the
+               prompt, the others generated (None: all of them generated)
+    penalties  float32 [T, 3]: repetition, frequency, presence (with tokens)
+    bias_ids   int64 [T, M], bias float32 [T, M]; of several entries of one id the
+               last counts
+    mask       int32 [T, ceil(V / 32)]: bit n % 32 of word n // 32 set where id n
+               is allowed
+    ids        int64 [T], written: the id of the largest allowed logit, the
+               smallest on ties, NaN counting as the largest, -1 where the mask
+               allows none
+
+    Ids outside [0, V), such as the -1 of an unused entry, are passed over.  All on
+    one GPU; nothing is read back, so a call can be captured in a HIP graph."""
+    if not torch.is_tensor(x) or not x.is_cuda:
+        raise ValueError("adjust: x must be a tensor on the GPU")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError("adjust: x must be [T, V]")
+    (T, V), dev = x.shape, x.device
+    out = x if out is None else out
+    xs, ys = _rows(x, "x", torch.float32, T, V, dev), _rows(out, "out", torch.float32, T, V, dev)
+    if T > 1 and ys < V:
+        raise ValueError("adjust: the rows of out must not overlap")
+    a = Rules()
+    if tokens is not None:
+        a.tokens_stride = _rows(tokens, "tokens", torch.int64, T, None, dev)
+        _vector(length, "length", torch.int32, T, dev)
+        if prompt is not None:
+            _vector(prompt, "prompt", torch.int32, T, dev)
+        if (not torch.is_tensor(penalties) or penalties.dtype != torch.float32 or tuple(penalties.shape) != (T, 3)
+                or not penalties.is_contiguous() or penalties.device != dev):
+            raise ValueError(f"adjust: penalties must be contiguous float32 [{T}, 3] on the device of x")
+        if tokens.shape[1]:
+            a.tokens, a.length, a.prompt, a.penalties = _ptr(tokens), _ptr(length), _ptr(prompt), _ptr(penalties)
+            a.max_tokens = tokens.shape[1]
+    elif length is not None or prompt is not None or penalties is not None:
+        raise ValueError("adjust: length, prompt and penalties go with tokens")
+    if bias_ids is not None or bias is not None:
+        a.bias_stride = _rows(bias_ids, "bias_ids", torch.int64, T, None, dev)
+        if _rows(bias, "bias", torch.float32, T, bias_ids.shape[1], dev) != a.bias_stride:
+            raise ValueError("adjust: bias_ids and bias must have one layout")
+        if bias_ids.shape[1]:
+            a.bias_ids, a.bias, a.n_bias = _ptr(bias_ids), _ptr(bias), bias_ids.shape[1]
+    if mask is not None:
+        a.mask_stride = _rows(mask, "mask", torch.int32, T, -(-V // 32), dev)
+        a.mask = _ptr(mask)
+    if ids is not None:
+        _vector(ids, "ids", torch.int64, T, dev)
+    if T == 0:
+        return out
+    L = lib()
+    with torch.cuda.device(dev):
+        need = L.rv12_logits_workspace_bytes(V, T) if ids is not None else 0
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        check(L.rv12_logits_adjust(ctypes.byref(a), _ptr(x), xs, _ptr(out), ys, V, T, _ptr(ids), _ptr(ws), need,
+                                   _stream(dev)), "adjust")
+    return out

@@ -37,6 +37,8 @@ enum rv12_status {
     RV12_E_SIZE = -9,      /* output buffer smaller than rv12_tiles_bytes() */
     RV12_E_SCRATCH = -10,  /* rv12_gemm_static: workspace beyond RV12_STATIC_SCRATCH_BYTES */
     RV12_E_PAGED = -11,    /* rv12_paged out of range, or t outside [1, 65536] */
+    RV12_E_RULES = -12,    /* rv12_rules: t, v, a count or a stride out of range */
+    RV12_E_LORA = -13,     /* rv12_lora or t out of range */
     RV12_E_LAUNCH = -20    /* hipGetLastError() after a launch */
 };
 
@@ -399,6 +401,68 @@ size_t rv12_paged_attend_workspace_bytes(const rv12_paged* a, int t);
 int rv12_paged_attend(const rv12_paged* a, int t, const float* q, const int32_t* seq, const int64_t* pos,
                       const int32_t* table, const void* kc, const void* vc, float* out, void* ws, size_t ws_bytes,
                       void* stream);
+
+/* Rules on the logits of t rows before the pick.  Per row, for every id n of v:
+ *   l' = l;  n among the row's tokens: l' = l > 0 ? l / repetition : l * repetition
+ *   n among its generated tokens, c times: l' -= frequency c + presence
+ *   n in bias_ids: l' += its bias (the last entry of an id)
+ *   n not allowed by the mask: l' = -inf, whatever l is
+ * in float32, in this order.  tokens: int64, the first length[r] (at most
+ * max_tokens, taken as 0 below) entries of row r, of which the first prompt[r]
+ * are the prompt (prompt NULL: all generated); penalties: float[t][3] =
+ * repetition, frequency, presence (NULL with tokens NULL); bias_ids / bias: n_bias
+ * entries per row; mask: bit n & 31 of word n >> 5 of the row set where id n is
+ * allowed.  Ids outside [0, v) in tokens and bias_ids are passed over.  Every
+ * part may be absent (NULL).  Strides are in elements, from row to row.  A field's
+ * rows may all be one (stride 0). */
+typedef struct rv12_rules {
+    const int64_t* tokens;
+    const int32_t* length;
+    const int32_t* prompt;
+    const float* penalties;
+    const int64_t* bias_ids;
+    const float* bias;
+    const uint32_t* mask;
+    int64_t tokens_stride, bias_stride, mask_stride;
+    int32_t max_tokens, n_bias;
+} rv12_rules;
+
+/* y[r] = the rules on x[r], 1 <= t <= 65535 rows of 1 <= v < 2^31 - 65536 logits
+ * (y may be x: each logit is read and written once).  ids: NULL, or int64[t] that
+ * receives the id of each row's largest y among the allowed ones, the smallest on
+ * ties, NaN counting as larger than any number, -1 where the mask allows none.
+ * ws: rv12_logits_workspace_bytes(v, t) bytes, 8-byte aligned, read only with ids.
+ * Stands beside rv12_head_argmax (the pick without rules); the reference applies
+ * its grammar masks on the host
+ * (ramvi/engine/ramvi_engine/generation/constrain.py). */
+size_t rv12_logits_workspace_bytes(int64_t v, int t);
+int rv12_logits_adjust(const rv12_rules* rules, const float* x, int64_t x_stride, float* y, int64_t y_stride, int64_t v,
+                       int t, int64_t* ids, void* ws, size_t ws_bytes, void* stream);
+
+/* A bank of low-rank adapters of one linear W[n, k]: a [count][r][k] and b
+ * [count][n][r] (bf16 bits, device), scale[count]; ranks[count] (NULL: r each): an
+ * adapter's entries from its rank on are not used, those of b must be finite.  r a
+ * multiple of 8 up to 128; k a multiple of 32. */
+typedef struct rv12_lora {
+    const uint16_t* a;
+    const uint16_t* b;
+    const float* scale;
+    const int32_t* ranks;
+    int32_t n, k, r, count;
+} rv12_lora;
+
+/* out[i] = y[i] + scale[j] b[j] (a[j] x'[i]), j = idx[i] (int32), for 1 <= t <=
+ * 65536 rows: the requests' own adapters beside the shared linear that left y.
+ * x (rows k floats apart, 2 k in mode 2) and x' as rv12_gemv: mode 0 or 1 x' = x,
+ * with lnw the RMSNorm; mode 2 x' = silu(x[0:k]) * x[k:2k] (no lnw).  A row whose
+ * idx is outside [0, count) has no adapter: out[i] = y[i].  out may be y (same
+ * stride); strides in floats.  Products of x', a, b and the sums between are
+ * float32 exact to rounding (three bf16 parts), finite x assumed.  Two passes, no
+ * atomics.  ws: rv12_lora_workspace_bytes(r, k, t) bytes, 16-byte aligned. */
+size_t rv12_lora_workspace_bytes(int r, int k, int t);
+int rv12_lora_apply(const rv12_lora* a, const float* x, const float* y, int64_t y_stride, float* out, int64_t out_stride,
+                    const int32_t* idx, int t, const uint16_t* lnw, float eps, int mode, void* ws, size_t ws_bytes,
+                    void* stream);
 
 #ifdef __cplusplus
 }
