@@ -7,6 +7,7 @@ the library is missing or does not match its build manifest (the sha256 of
 the binary and of every source, the flags, the ABI version: ai_amd/build.py);
 there is no fallback path.
 """
+import contextlib
 import ctypes
 import os
 
@@ -185,6 +186,15 @@ def lib():
             raise RuntimeError(f"librv12.so ABI version {v}, expected {ABI_VERSION}")
         _lib = L
     return _lib
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on(device):
+    """The device of a call's tensors as the current one (a launch goes to the
+    current device, whatever its stream); nothing to do where it is already."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def strerror(status):

@@ -12,14 +12,8 @@ import ctypes
 
 import torch
 
-from ._lib import Attn, Paged, check, lib
+from ._lib import Attn, Paged, check, lib, on
 from .wcomp import _ptr, _stream
-
-
-def _on(dev):
-    """The device of a call's tensors as the current one: a launch goes to the
-    current device, whatever its stream."""
-    return torch.cuda.device(dev)
 
 
 SPAN = 80  # positions one workgroup covers at most
@@ -150,76 +144,84 @@ class PagedRopeAttn:
         self.n_heads, self.n_kv, self.head_dim, self.page = (int(v) for v in (n_heads, n_kv, head_dim, page))
         self.eps = float(eps)
         self.scale = float(self.head_dim ** -0.5 if scale is None else scale)
-        a = self._struct(1, 1, 1, 1)
-        if lib().rv12_paged_attend_workspace_bytes(ctypes.byref(a), 1) == 0:
+        self._page_shape = (self.n_kv, self.page, self.head_dim)
+        self._structs = {}  # sizes of the table and the caches -> argument struct
+        if lib().rv12_paged_attend_workspace_bytes(self._struct(1, 1, 1, 1), 1) == 0:
             raise ValueError("paged attention: head_dim must be 64 or 128, n_heads 1 to 16 times n_kv, page a power of "
                              "two from 16 to 1024")
 
-    def _struct(self, n_seq, max_pages, stride, n_pages):
-        return Paged(self.n_heads, self.n_kv, self.head_dim, self.page, 1 if self.kv_dtype == torch.bfloat16 else 0,
-                     n_seq, max_pages, stride, n_pages, self.eps, self.scale)
+    def _struct(self, *sizes):
+        """The argument struct of n_seq, max_pages, table_stride, n_pages."""
+        a = self._structs.get(sizes)
+        if a is None:
+            if len(self._structs) >= 256:
+                self._structs.clear()
+            a = self._structs[sizes] = ctypes.byref(Paged(
+                self.n_heads, self.n_kv, self.head_dim, self.page, 1 if self.kv_dtype == torch.bfloat16 else 0, *sizes,
+                self.eps, self.scale))
+        return a
 
-    def _rows(self, rows, seq, pos, table, kc, vc):
+    def _rows(self, dev, rows, seq, pos, table, kc, vc):
         """The argument struct of a call and its row count; rows: (tensor,
-        floats of one row) pairs."""
-        first = rows[0][0]
-        if not first.is_cuda:
+        floats of one row) pairs.  dev: index of the GPU."""
+        if dev < 0:
             raise ValueError("the tensors must be on the GPU")
-        dev = first.device
         T = pos.numel()
-        if pos.dtype != torch.int64 or pos.dim() != 1 or not pos.is_contiguous() or pos.device != dev:
+        if pos.dtype != torch.int64 or pos.dim() != 1 or not pos.is_contiguous() or pos.get_device() != dev:
             raise ValueError("pos must be a contiguous int64 vector on the rows' device")
-        if seq is not None and (seq.dtype != torch.int32 or seq.shape != pos.shape or not seq.is_contiguous()
-                                or seq.device != dev):
-            raise ValueError("seq must be an int32 vector with an entry for every row, on the rows' device")
+        if seq is not None and (seq.dtype != torch.int32 or seq.dim() != 1 or seq.numel() != T
+                                or not seq.is_contiguous() or seq.get_device() != dev):
+            raise ValueError("seq must be a contiguous int32 vector with an entry for every row, on the rows' device")
         for t, n in rows:
-            if t.dtype != torch.float32 or not t.is_contiguous() or t.device != dev or t.numel() != T * n:
+            if t.dtype != torch.float32 or t.numel() != T * n or not t.is_contiguous() or t.get_device() != dev:
                 raise ValueError(f"qkv, q and out must be contiguous float32 with {T} rows, on one device")
-        if (table.dtype != torch.int32 or table.dim() != 2 or table.device != dev or table.stride(1) != 1
-                or min(table.shape) < 1):
-            raise ValueError("table must be int32 [sequences, pages], its rows contiguous, on the rows' device")
-        for c in (kc, vc):
-            if (c.dtype != self.kv_dtype or not c.is_contiguous() or c.device != dev or c.dim() != 4
-                    or tuple(c.shape[1:]) != (self.n_kv, self.page, self.head_dim) or c.shape != kc.shape):
-                raise ValueError(f"kc and vc must be contiguous {self.kv_dtype} caches of shape "
-                                 f"(pages, {self.n_kv}, {self.page}, {self.head_dim})")
+        if table.dtype != torch.int32 or table.dim() != 2 or table.get_device() != dev:
+            raise ValueError("table must be int32 [sequences, pages], on the rows' device")
         n_seq, max_pages = table.shape
-        stride = table.stride(0) if n_seq > 1 else max_pages
-        if stride < max_pages:
-            raise ValueError("the table's rows must not overlap")
-        return self._struct(n_seq, max_pages, stride, kc.shape[0]), T
+        stride, one = table.stride()
+        if n_seq == 1:
+            stride = max_pages
+        if n_seq < 1 or max_pages < 1 or (one != 1 and max_pages > 1) or stride < max_pages:
+            raise ValueError("the table's rows must be contiguous, not empty and not overlap")
+        n_pages = kc.shape[0]
+        want, shape = self.kv_dtype, (n_pages,) + self._page_shape
+        if (kc.dtype != want or vc.dtype != want or kc.shape != shape or vc.shape != shape or not kc.is_contiguous()
+                or not vc.is_contiguous() or kc.get_device() != dev or vc.get_device() != dev):
+            raise ValueError(f"kc and vc must be contiguous {want} caches of shape "
+                             f"(pages, {self.n_kv}, {self.page}, {self.head_dim})")
+        return self._struct(n_seq, max_pages, stride, n_pages), T
 
     def append(self, qkv, qn, kn, inv, seq, pos, table, kc, vc, q):
         """Head norms and rotation of the rows' q and k: q to q, k and v to
         their pages."""
-        a, T = self._rows([(qkv, (self.n_heads + 2 * self.n_kv) * self.head_dim), (q, self.n_heads * self.head_dim)],
+        dev = qkv.get_device()
+        a, T = self._rows(dev, ((qkv, (self.n_heads + 2 * self.n_kv) * self.head_dim), (q, self.n_heads * self.head_dim)),
                           seq, pos, table, kc, vc)
         for t, n in ((qn, self.head_dim), (kn, self.head_dim), (inv, self.head_dim // 2)):
-            if t.dtype != torch.float32 or not t.is_contiguous() or t.device != qkv.device or t.numel() != n:
+            if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous() or t.get_device() != dev:
                 raise ValueError("qn, kn and inv must be contiguous float32 of head_dim, head_dim and head_dim / 2 "
                                  "entries, on the rows' device")
         if T == 0:
             return
-        with _on(qkv.device):
-            check(lib().rv12_paged_append(ctypes.byref(a), T, _ptr(qkv), _ptr(qn), _ptr(kn), _ptr(inv), _ptr(seq),
-                                          _ptr(pos), _ptr(table), _ptr(kc), _ptr(vc), _ptr(q), _stream(qkv.device)),
-                  "paged_append")
+        with on(qkv.device):
+            check(lib().rv12_paged_append(a, T, _ptr(qkv), _ptr(qn), _ptr(kn), _ptr(inv), _ptr(seq), _ptr(pos),
+                                          _ptr(table), _ptr(kc), _ptr(vc), _ptr(q), _stream(qkv.device)), "paged_append")
 
     def attend(self, q, seq, pos, table, kc, vc, out):
         """The attention of the rows (q as append leaves it) over their
         sequences' positions 0 .. pos, the rows' own among them."""
         n = self.n_heads * self.head_dim
-        a, T = self._rows([(q, n), (out, n)], seq, pos, table, kc, vc)
+        a, T = self._rows(q.get_device(), ((q, n), (out, n)), seq, pos, table, kc, vc)
         if T == 0:
             return
         L = lib()
-        with _on(q.device):
-            need = L.rv12_paged_attend_workspace_bytes(ctypes.byref(a), T)
+        with on(q.device):
+            need = L.rv12_paged_attend_workspace_bytes(a, T)
             if need == 0:
                 raise ValueError("paged attention: too many rows or positions")
             ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-            check(L.rv12_paged_attend(ctypes.byref(a), T, _ptr(q), _ptr(seq), _ptr(pos), _ptr(table), _ptr(kc),
-                                      _ptr(vc), _ptr(out), _ptr(ws), need, _stream(q.device)), "paged_attend")
+            check(L.rv12_paged_attend(a, T, _ptr(q), _ptr(seq), _ptr(pos), _ptr(table), _ptr(kc), _ptr(vc), _ptr(out),
+                                      _ptr(ws), need, _stream(q.device)), "paged_attend")
 
     def __call__(self, qkv, qn, kn, inv, seq, pos, table, kc, vc, out):
         """append, then attend."""

@@ -811,8 +811,9 @@ static int paged_params(const rv12_paged* a, int t, PagedParams* p) {
     p->cap = cap;
     p->eps = a->eps;
     p->scale = a->scale;
-    // the plan's chunk length stays an int
-    if ((double)t * (double)cap * a->n_kv / p->target > (double)(1 << 30)) return RV12_E_PAGED;
+    // the plan's sum of 32-position blocks and its chunk length stay ints
+    if ((int64_t)t * cap > (int64_t)1 << 35 || (int64_t)t * cap / p->target * a->n_kv > (int64_t)1 << 30) return RV12_E_PAGED;
+    p->grain = p->kv_bf16 ? 128 : 64;
     return RV12_OK;
 }
 
@@ -843,7 +844,7 @@ int rv12_paged_append(const rv12_paged* a, int t, const float* qkv, const float*
 size_t rv12_paged_attend_workspace_bytes(const rv12_paged* a, int t) {
     PagedParams p;
     if (paged_params(a, t, &p)) return 0;
-    return 16 + (size_t)paged_slots(p) * p.n_kv * (p.rt * p.g) * (p.head_dim + 2) * 4;
+    return 16 + (size_t)paged_slots(p) * p.n_kv * (p.rt * p.g) * (p.head_dim + 4) * 4;
 }
 
 int rv12_paged_attend(const rv12_paged* a, int t, const float* q, const int32_t* seq, const int64_t* pos,

@@ -189,7 +189,8 @@ struct PagedParams {
     int T, n_heads, n_kv, head_dim, kv_bf16, page_log, n_seq;
     int g;   // query heads per kv head
     int rt;  // rows of one sequence that share a workgroup's 16 columns at most
-    int target = 1024, min_chunk = 128;
+    int target = 1024;      // workgroups that share the positions
+    int grain = 128;    // chunk lengths are multiples of this (a power of two): one step of a workgroup's waves
     int64_t table_stride, n_pages, cap;  // cap: positions the table covers
     float eps, scale;
 };
@@ -197,12 +198,11 @@ constexpr int kMaxPagedRows = 1 << 16;
 // workgroups per kv head at most: every row has a chunk, and rows of n > C
 // positions have fewer than n / C + 1, the sum of n being at most C target / n_kv
 inline int64_t paged_items(const PagedParams& p) {
-    const int64_t c = (p.min_chunk + 127) / 128 * 128;
-    return std::min((int64_t)p.target / p.n_kv + p.T, (int64_t)p.T * ((p.cap + c - 1) / c));
+    return std::min((int64_t)p.target / p.n_kv + p.T, (int64_t)p.T * ((p.cap + p.grain - 1) / p.grain));
 }
 // rows of several chunks at most (n > C each), and their chunks (fewer than 2 n / C each)
 inline int paged_split_rows(const PagedParams& p) {
-    return p.cap <= (p.min_chunk + 127) / 128 * 128 ? 0 : std::min(p.T, p.target / p.n_kv);
+    return p.cap <= p.grain ? 0 : std::min(p.T, p.target / p.n_kv);
 }
 inline int paged_slots(const PagedParams& p) { return paged_split_rows(p) ? 2 * (p.target / p.n_kv) : 0; }
 void launch_paged_append(const PagedParams& p, hipStream_t st);

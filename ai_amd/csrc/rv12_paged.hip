@@ -13,6 +13,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "rv12_device.h"
 #include "rv12_internal.h"
 
@@ -175,88 +177,128 @@ struct PlanRows {
     int nr, n;
 };
 
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ int dpp_int(int v) {  // 0 where no lane is named
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+constexpr int kDppDown1 = 0x101, kDppDown2 = 0x102, kDppDown4 = 0x104, kDppDown8 = 0x108;  // lane i gets i + n of its 16
+constexpr int kDppUp1 = 0x111, kDppUp2 = 0x112, kDppUp4 = 0x114, kDppUp8 = 0x118;          // i - n
+// inclusive sum over the wave's lanes
+__device__ __forceinline__ int wave_scan(int v) {
+    v += dpp_int<kDppUp1>(v);
+    v += dpp_int<kDppUp2>(v);
+    v += dpp_int<kDppUp4>(v);
+    v += dpp_int<kDppUp8>(v);
+    v += dpp_int<0x142, 0xA>(v);  // lane 15 of rows 0 and 2 to the row after
+    v += dpp_int<0x143, 0xC>(v);  // lane 31 to rows 2 and 3
+    return v;
+}
+
 __device__ __forceinline__ PlanRows plan_rows(const PagedParams& p, int base) {
     const int lane = threadIdx.x & 63, r = base + lane;
     int key = -1 - r, n = 0;  // rows without a sequence share nothing
     if (r < p.T) {
-        const int64_t sq = p.seq ? (int64_t)p.seq[r] : r;
         const int64_t pos = p.pos[r];
+        const int64_t sq = p.seq ? (int64_t)p.seq[r] : r;
         if (sq >= 0 && sq < p.n_seq) {
             key = (int)sq;
             if (pos >= 0 && pos < p.cap) n = (int)pos + 1;
         }
     }
+    // tiles are aligned to rt <= 16 rows, so a tile stays within 16 lanes
+    const int before = dpp_int<kDppUp1>(key);  // (every lane active: no part of a condition)
+    const bool joins = r < p.T && (r & (p.rt - 1)) != 0 && before == key;
+    const uint64_t m = __ballot(joins);
     PlanRows o;
-    const int before = __shfl_up(key, 1), in_tile = r & (p.rt - 1);
-    o.leader = r < p.T && (in_tile == 0 || before != key);
+    o.leader = r < p.T && !joins;
     o.nr = 1;
     o.n = n;
-    bool same = true;
-    for (int j = 1; j < p.rt; ++j) {
-        const int k2 = __shfl_down(key, j), n2 = __shfl_down(n, j);
-        same = same && in_tile + j < p.rt && lane + j < 64 && k2 == key;
-        if (same) {
-            ++o.nr;
-            o.n = max(o.n, n2);
-        }
+    if (m) {
+        o.nr = 1 + __builtin_ctzll(~((m >> lane) >> 1));
+        int k;
+        k = dpp_int<kDppDown1>(o.n);
+        if (o.nr > 1) o.n = max(o.n, k);
+        k = dpp_int<kDppDown2>(o.n);
+        if (o.nr > 2) o.n = max(o.n, k);
+        k = dpp_int<kDppDown4>(o.n);
+        if (o.nr > 4) o.n = max(o.n, k);
+        k = dpp_int<kDppDown8>(o.n);
+        if (o.nr > 8) o.n = max(o.n, k);
     }
     return o;
 }
 
-// chunk length of the plan: all positions over the target, in steps of 128
-__device__ __forceinline__ int plan_chunk(const PagedParams& p) {
-    int64_t total = 0;
-    for (int base = 0; base < p.T; base += 64) {
-        const PlanRows o = plan_rows(p, base);
-        total += o.leader ? o.n : 0;
-    }
-#pragma unroll
-    for (int j = 1; j < 64; j <<= 1) total += __shfl_xor(total, j);
-    const int64_t c = (total * p.n_kv + p.target - 1) / p.target;
-    return (int)(max(c, (int64_t)p.min_chunk) + 127) & ~127;
-}
-
 struct PlanItem {
     int row, nr, n;     // leader row, rows, positions
+    int C;              // chunk length
     int chunk, chunks;  // of this row
     int slot;           // first partial of the row (rows of several chunks only)
 };
 
-// item `want` among the chunks of all rows; `several` true: row `want` among the
-// rows of several chunks.  False if there is none.
-__device__ __forceinline__ bool plan_find(const PagedParams& p, int C, int want, bool several, PlanItem* it) {
-    const int lane = threadIdx.x & 63;
+// item `want` among the chunks of all rows, or (SEVERAL) row `want` among the rows
+// of several chunks.  False if there is none.  The chunk length: all positions
+// (in blocks of 32) over the target, in grains (one step of every wave).
+template <bool SEVERAL>
+__device__ __forceinline__ bool plan_find(const PagedParams& p, int want, PlanItem* it) {
+    const PlanRows r0 = plan_rows(p, 0);
+    int total = __builtin_amdgcn_readlane(wave_scan(r0.leader ? (r0.n + 31) >> 5 : 0), 63);
+    for (int base = 64; base < p.T; base += 64) {
+        const PlanRows o = plan_rows(p, base);
+        total += __builtin_amdgcn_readlane(wave_scan(o.leader ? (o.n + 31) >> 5 : 0), 63);
+    }
+    // up to 512 positions a chunk's own cost counts, and one workgroup per resident
+    // slot is best; above it smaller chunks even out the workgroups' ends
+    // (1024 target: 8 rows of one sequence at 4096 positions, 64 query heads over 8,
+    // 18.9 -> 16.9 us with half the workgroups; 64 rows of 500 to 8200 positions, 32
+    // heads over 8, 142 us, 155 with half)
+    const int64_t all = (int64_t)total * p.n_kv;
+    const int64_t half_c = (all + p.target / 2 - 1) / (p.target / 2) * 32;
+    const int64_t c = half_c <= 512 ? half_c : max((all + p.target - 1) / p.target * 32, (int64_t)512);
+    const int C = (int)((max(c, (int64_t)1) + p.grain - 1) & ~(int64_t)(p.grain - 1));
     int items0 = 0, slots0 = 0;
     for (int base = 0; base < p.T; base += 64) {
-        const PlanRows o = plan_rows(p, base);
+        const PlanRows o = base ? plan_rows(p, base) : r0;
         const int ch = o.leader ? max(1, (o.n + C - 1) / C) : 0;
         const int sl = ch > 1 ? ch : 0;
-        const int mine = several ? (ch > 1 ? 1 : 0) : ch;
-        int items = mine, slots = sl;
-#pragma unroll
-        for (int j = 1; j < 64; j <<= 1) {
-            const int a = __shfl_up(items, j), b = __shfl_up(slots, j);
-            if (lane >= j) {
-                items += a;
-                slots += b;
-            }
-        }
-        const int e = items0 + items - mine;
+        const int mine = SEVERAL ? (ch > 1 ? 1 : 0) : ch;
+        // both sums at once: at most 2 target slots and target / n_kv + T items
+        const int both = wave_scan(sl << 18 | mine);
+        const int e = items0 + (both & 0x3FFFF) - mine;
         const uint64_t hit = __ballot(want >= e && want < e + mine);
         if (hit) {
             const int s = __builtin_ctzll(hit);
             it->row = base + s;
             it->nr = __builtin_amdgcn_readlane(o.nr, s);
             it->n = __builtin_amdgcn_readlane(o.n, s);
+            it->C = C;
             it->chunk = want - __builtin_amdgcn_readlane(e, s);
             it->chunks = __builtin_amdgcn_readlane(ch, s);
-            it->slot = slots0 + __builtin_amdgcn_readlane(slots - sl, s);
+            it->slot = slots0 + __builtin_amdgcn_readlane((both >> 18) - sl, s);
             return true;
         }
-        items0 += __builtin_amdgcn_readlane(items, 63);
-        slots0 += __builtin_amdgcn_readlane(slots, 63);
+        const int last = __builtin_amdgcn_readlane(both, 63);
+        items0 += last & 0x3FFFF;
+        slots0 += last >> 18;
     }
     return false;
+}
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+// split3 with a pair of values per conversion
+__device__ __forceinline__ uint32_t bf16_pair(f32x2 v) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+}
+__device__ __forceinline__ void split3_pairs(const float (&v)[8], u32x4& hi, u32x4& mid, u32x4& lo) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        f32x2 a = {v[2 * j], v[2 * j + 1]};
+        hi[j] = bf16_pair(a);
+        a = f32x2{a.x - lo_f(hi[j]), a.y - hi_f(hi[j])};
+        mid[j] = bf16_pair(a);
+        a = f32x2{a.x - lo_f(mid[j]), a.y - hi_f(mid[j])};
+        lo[j] = bf16_pair(a);
+    }
 }
 
 __device__ __forceinline__ float max4rows(float v) {
@@ -266,13 +308,13 @@ __device__ __forceinline__ float sum4rows(float v) {
     return rows_and_halves(v, [](float x, float y) { return x + y; });
 }
 
-// partial p of kv head g: [columns][HD + 2]
+// the partial of a slot and kv head: [columns][HD + 4], the sums, m and l
 __device__ __forceinline__ float* paged_part(const PagedParams& p, int HD, int slot, int g) {
-    return p.part + ((int64_t)slot * p.n_kv + g) * (p.rt * p.g) * (HD + 2);
+    return p.part + ((int64_t)slot * p.n_kv + g) * (p.rt * p.g) * (HD + 4);
 }
 
-template <int HD, bool BF16>
-__global__ __launch_bounds__(256, 2) void k_paged_attend(PagedParams p) {
+template <int HD, bool BF16, bool ONCE>
+__global__ __launch_bounds__(256, 3) void k_paged_attend(PagedParams p) {
     constexpr int EB = BF16 ? 2 : 4;   // cache bytes per value
     constexpr int NB = BF16 ? 2 : 1;   // blocks of 16 positions per step
     constexpr int PB = 16 * NB;
@@ -282,16 +324,26 @@ __global__ __launch_bounds__(256, 2) void k_paged_attend(PagedParams p) {
     constexpr int VW = DT * EB / 4;    // words of one lane's value dims
     constexpr int NW = 4;              // waves
     constexpr int ROWB = HD * EB;      // bytes of one position
+    constexpr int kPolicy = ONCE ? kNonTemporal : 0;
     __shared__ float lds[NW * (DT * 256 + 128)];
+    __shared__ u32x4 qp[BF16 ? NA : 1][3][BF16 ? 64 : 1];
+    __shared__ f32x4 qf[BF16 ? 1 : NA][2][BF16 ? 1 : 64];
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q4 = lane >> 4, c16 = lane & 15;
     const int g = blockIdx.x % p.n_kv, item = blockIdx.x / p.n_kv;
     const int G = p.g, H = p.n_heads;
 
-    const int C = plan_chunk(p);
     PlanItem it;
-    if (!plan_find(p, C, item, false, &it)) return;
+    if (!plan_find<false>(p, item, &it)) return;
+    // (said to be uniform, so that the loads' descriptors stay in scalar registers)
+    it.row = __builtin_amdgcn_readfirstlane(it.row);
+    it.nr = __builtin_amdgcn_readfirstlane(it.nr);
+    it.n = __builtin_amdgcn_readfirstlane(it.n);
+    it.C = __builtin_amdgcn_readfirstlane(it.C);
+    it.chunk = __builtin_amdgcn_readfirstlane(it.chunk);
+    it.chunks = __builtin_amdgcn_readfirstlane(it.chunks);
+    it.slot = __builtin_amdgcn_readfirstlane(it.slot);
 
     // this lane's column: head cg of row r0 + rt
     const int rt = c16 / G, cg = c16 - rt * G;
@@ -299,33 +351,29 @@ __global__ __launch_bounds__(256, 2) void k_paged_attend(PagedParams p) {
     const int row = it.row + (col ? rt : 0);
     const int64_t prow = p.pos[row];
     const int lim = col && it.n > 0 && prow >= 0 && prow < p.cap ? (int)prow : -1;  // last position it sees
-    const int lo = it.chunk * C, hi = min(it.n, lo + C);
+    const int lo = it.chunk * it.C, hi = min(it.n, lo + it.C);
     const int64_t sq = p.seq ? (int64_t)p.seq[it.row] : it.row;
     // the smallest of the columns' limits: up to it every column sees every position
-    int first = col ? lim : 0x7FFFFFFF;
+    int first = it.n - 1;
+    if (it.nr > 1) {
+        first = col ? lim : 0x7FFFFFFF;
 #pragma unroll
-    for (int j = 1; j < 16; j <<= 1) first = min(first, __shfl_xor(first, j));
+        for (int j = 1; j < 16; j <<= 1) first = min(first, __shfl_xor(first, j));
+    }
     first = __builtin_amdgcn_readfirstlane(first);
 
-    // q of the column, times scale log2(e): the scores are exponents of 2
-    float qv[NA][8];
-    {
-        const float* src = p.q + ((int64_t)row * H + g * G + cg) * HD + 8 * q4;
-        const float f = p.scale * 1.44269504088896341f;
+    // q of the column: wave w loads the 8-dim chunks w, w + 4, .., before anything
+    // waits
+    constexpr int QC = (NA + NW - 1) / NW;
+    f32x4 qin[QC][2];
 #pragma unroll
-        for (int a = 0; a < NA; ++a)
+    for (int i = 0; i < QC; ++i) {
+        const float* src = p.q + ((int64_t)row * H + g * G + cg) * HD + 8 * q4 + 32 * (wv + NW * i);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                f32x4 v = {0, 0, 0, 0};
-                if (col) v = *reinterpret_cast<const f32x4*>(src + 32 * a + 4 * c);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) qv[a][4 * c + e] = v[e] * f;
-            }
-    }
-    u32x4 qp[BF16 ? NA : 1][3];
-    if constexpr (BF16) {
-#pragma unroll
-        for (int a = 0; a < NA; ++a) split3(qv[a], qp[a][0], qp[a][1], qp[a][2]);
+        for (int c = 0; c < 2; ++c) {
+            qin[i][c] = f32x4{0, 0, 0, 0};
+            if (col && wv + NW * i < NA) qin[i][c] = *reinterpret_cast<const f32x4*>(src + 4 * c);
+        }
     }
 
     f32x4 o[DT];
@@ -344,13 +392,16 @@ __global__ __launch_bounds__(256, 2) void k_paged_attend(PagedParams p) {
         if (ids >= p.n_pages) ids = -1;
     };
     uint32_t kw[NB][NA][KW], vw[NB][4][VW];
+    const int koff = c16 * ROWB + 8 * q4 * EB, voff = 4 * q4 * ROWB + DT * c16 * EB;
     // descriptor of block b of step s (k: kc or vc): its positions below hi
     auto block = [&](const void* cache, int s, int b, int id) {
         const int ps = lo + s * PB + 16 * b;
         const int rows = id < 0 ? 0 : min(16, hi - ps);
         const int64_t off =
             ((((int64_t)max(id, 0) * p.n_kv + g) << p.page_log) + (ps & ((1 << p.page_log) - 1))) * ROWB;
-        return make_rsrc(static_cast<const char*>(cache) + off, (uint32_t)max(rows, 0) * ROWB);
+        // (a clamp is a vector instruction: back to a scalar register)
+        return make_rsrc(static_cast<const char*>(cache) + off,
+                         (uint32_t)__builtin_amdgcn_readfirstlane(max(rows, 0) * ROWB));
     };
     auto load_k = [&](int s, const int (&id)[NB]) {
 #pragma unroll
@@ -360,7 +411,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attend(PagedParams p) {
             for (int a = 0; a < NA; ++a)
 #pragma unroll
                 for (int c = 0; c < KW / 4; ++c) {
-                    const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, c16 * ROWB + (32 * a + 8 * q4) * EB + c * 16, 0, 0);
+                    const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, koff, 32 * a * EB + c * 16, kPolicy);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) kw[b][a][4 * c + e] = v[e];
                 }
@@ -372,15 +423,14 @@ __global__ __launch_bounds__(256, 2) void k_paged_attend(PagedParams p) {
             const __amdgpu_buffer_rsrc_t r = block(p.vc, s, b, id[b]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int off = (4 * q4 + j) * ROWB + DT * c16 * EB;
                 if constexpr (VW == 2) {
-                    const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
+                    const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, voff, j * ROWB, kPolicy);
                     vw[b][j][0] = v[0];
                     vw[b][j][1] = v[1];
                 } else {
 #pragma unroll
                     for (int c = 0; c < VW / 4; ++c) {
-                        const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, off + c * 16, 0, 0);
+                        const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, voff, j * ROWB + c * 16, kPolicy);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) vw[b][j][4 * c + e] = v[e];
                     }
@@ -393,32 +443,58 @@ __global__ __launch_bounds__(256, 2) void k_paged_attend(PagedParams p) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) id[b] = __builtin_amdgcn_readlane(ids, (k % SPR) * NB + b);
     };
-    // o[d] += V^T P^T over the step's positions
-    auto values = [&](const uint32_t (&w)[NB][4][VW], const float (&pr)[NB][4], f32x4 (&acc)[DT]) {
+    // o[d] += V^T P^T over the step's positions; MASKED: the positions past lm as
+    // zeros, and only the columns of row rr
+    auto values = [&](const float (&pr)[NB][4], auto masked, int p0, int lm, int rr) {
+        constexpr bool MASKED = decltype(masked)::value;
         if constexpr (BF16) {
             float p8[8];
+            uint32_t keep[4];
 #pragma unroll
             for (int j = 0; j < 8; ++j) p8[j] = pr[j >> 2][j & 3];
             u32x4 ph, pm, pl;
-            split3(p8, ph, pm, pl);
+            split3_pairs(p8, ph, pm, pl);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int ps = p0 + 16 * (j >> 1) + 4 * q4 + 2 * (j & 1);
+                keep[j] = (ps <= lm ? 0xFFFFu : 0u) | (ps + 1 <= lm ? 0xFFFF0000u : 0u);
+            }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 // the same dim of the 4 + 4 positions: two 16-bit picks per word
                 u32x4 va;
                 const uint32_t sel = (d & 1) ? 0x07060302u : 0x05040100u;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    va[j] = __builtin_amdgcn_perm(w[j >> 1][2 * (j & 1) + 1][d >> 1], w[j >> 1][2 * (j & 1)][d >> 1], sel);
-                acc[d] = mfma(va, ph, acc[d]);
-                acc[d] = mfma(va, pm, acc[d]);
-                acc[d] = mfma(va, pl, acc[d]);
+                for (int j = 0; j < 4; ++j) {
+                    va[j] = __builtin_amdgcn_perm(vw[j >> 1][2 * (j & 1) + 1][d >> 1], vw[j >> 1][2 * (j & 1)][d >> 1], sel);
+                    if constexpr (MASKED) va[j] &= keep[j];
+                }
+                f32x4 t = mfma(va, ph, o[d]);
+                t = mfma(va, pm, t);
+                t = mfma(va, pl, t);
+                if constexpr (MASKED) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[d][r] = rt == rr ? t[r] : o[d][r];
+                } else {
+                    o[d] = t;
+                }
             }
         } else {
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+            for (int d = 0; d < DT; ++d) {
+                f32x4 t = o[d];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(word_f(w[0][j], d), pr[0][j], acc[d], 0, 0, 0);
+                for (int j = 0; j < 4; ++j) {
+                    const float v = !MASKED || p0 + 4 * q4 + j <= lm ? word_f(vw[0][j], d) : 0.0f;
+                    t = __builtin_amdgcn_mfma_f32_16x16x4f32(v, pr[0][j], t, 0, 0, 0);
+                }
+                if constexpr (MASKED) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[d][r] = rt == rr ? t[r] : o[d][r];
+                } else {
+                    o[d] = t;
+                }
+            }
         }
     };
 
@@ -427,10 +503,38 @@ __global__ __launch_bounds__(256, 2) void k_paged_attend(PagedParams p) {
         refill(wv);
         ids_of(0, id);
         load_k(wv, id);
+        // keys before values, as in the loop: its first wait is then for the keys alone
+        __builtin_amdgcn_sched_barrier(0);
         load_v(wv, id);
     }
-    for (int s = wv, k = 0; s < steps; s += NW, ++k) {
+    // q times scale log2(e) (the scores are exponents of 2) stays in LDS (bf16
+    // caches: its three parts), the same for the four waves: 48 (float32: 32)
+    // registers less, a third workgroup on every CU
+#pragma unroll
+    for (int i = 0; i < QC; ++i) {
+        const int a = wv + NW * i;
+        if (a >= NA) continue;
+        const float f = p.scale * 1.44269504088896341f;
+        qin[i][0] *= f;
+        qin[i][1] *= f;
+        if constexpr (BF16) {
+            float v8[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v8[e] = qin[i][e >> 2][e & 3];
+            u32x4 h, m, l;
+            split3_pairs(v8, h, m, l);
+            qp[a][0][lane] = h;
+            qp[a][1][lane] = m;
+            qp[a][2][lane] = l;
+        } else {
+            qf[a][0][lane] = qin[i][0];
+            qf[a][1][lane] = qin[i][1];
+        }
+    }
+    __syncthreads();
+    auto step = [&](int s, int k, auto apart) {
         const int p0 = lo + s * PB;
+        asm volatile("" ::: "memory");  // q is read again, not kept in registers
         // scores of positions p0 + 16 b + 4 q4 + r for the lane's column
         f32x4 sc[NB];
 #pragma unroll
@@ -441,11 +545,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_attend(PagedParams p) {
                 if constexpr (BF16) {
                     const u32x4 ka = {kw[b][a][0], kw[b][a][1], kw[b][a][2], kw[b][a][3]};
 #pragma unroll
-                    for (int c = 0; c < 3; ++c) acc = mfma(ka, qp[a][c], acc);
+                    for (int c = 0; c < 3; ++c) acc = mfma(ka, qp[a][c][lane], acc);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(word_f(kw[b][a], e), qv[a][e], acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(word_f(kw[b][a], e), qf[a][e >> 2][lane][e & 3], acc, 0, 0, 0);
                 }
             }
             sc[b] = acc;
@@ -453,12 +557,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_attend(PagedParams p) {
         int cur[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) cur[b] = id[b];
-        const bool more = s + NW < steps;
-        if (more) {
-            if ((k + 1) % SPR == 0) refill(s + NW);
-            ids_of(k + 1, id);
-            load_k(s + NW, id);
-        }
+        // the next step's keys; past the last step the ids are -1, and the loads
+        // read zeros without an access (no branch, so that each wait below is for
+        // the loads that it needs alone)
+        if ((k + 1) % SPR == 0) refill(s + NW);
+        ids_of(k + 1, id);
+        load_k(s + NW, id);
         float pr[NB][4];
         float mb = -INFINITY;
 #pragma unroll
@@ -488,36 +592,24 @@ __global__ __launch_bounds__(256, 2) void k_paged_attend(PagedParams p) {
                 pr[b][r] = __builtin_amdgcn_exp2f(pr[b][r] - mr);
                 l += pr[b][r];
             }
-        if (it.nr == 1 || p0 + PB - 1 <= first) {
-            values(vw, pr, o);
+        if constexpr (decltype(apart)::value) {
+            for (int rr = 0; rr < it.nr; ++rr)
+                values(pr, std::true_type{}, p0, __builtin_amdgcn_readlane(lim, rr * G), rr);
         } else {
-            // the columns' limits differ within these positions: per row, the values
-            // past its limit as zeros, so that one row's NaN or infinity does not meet
-            // another row's probability of 0
-            for (int rr = 0; rr < it.nr; ++rr) {
-                const int lm = __builtin_amdgcn_readlane(lim, rr * G);
-                uint32_t w[NB][4][VW];
-                f32x4 t[DT];
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int i = 0; i < VW; ++i) w[b][j][i] = p0 + 16 * b + 4 * q4 + j <= lm ? vw[b][j][i] : 0u;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) t[d] = o[d];
-                values(w, pr, t);
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[d][r] = rt == rr ? t[d][r] : o[d][r];
-            }
+            values(pr, std::false_type{}, 0, 0, 0);
         }
-        if (more) load_v(s + NW, id);
-    }
+        load_v(s + NW, id);
+    };
+    int s = wv, k = 0;
+    // the steps that every column sees whole (with one row: all), then those within
+    // which the columns' limits differ: per row, the values past its limit as zeros,
+    // so that one row's NaN or infinity does not meet another row's probability of 0
+    const int whole_steps = it.nr == 1 ? steps : min(steps, max(first + 1 - lo, 0) / PB);
+    for (; s < whole_steps; s += NW, ++k) step(s, k, std::false_type{});
+    for (; s < steps; s += NW, ++k) step(s, k, std::true_type{});
     l = sum4rows(l);
 
-    // join of the waves: wave w adds the sums of tiles d = w, w + 4, ..
+    // join of the waves: wave w adds the sums of its quarter of the tiles
     constexpr int kPart = DT * 256 + 128;
     float* mine = lds + wv * kPart;
 #pragma unroll
@@ -541,67 +633,89 @@ __global__ __launch_bounds__(256, 2) void k_paged_attend(PagedParams p) {
     if (!col) return;
     const bool whole = it.chunks == 1;
     const float inv_l = lj == 0.0f ? 0.0f : 1.0f / lj;  // nothing to attend: zeros
-    float* part = paged_part(p, HD, it.slot + it.chunk, g) + c16 * (HD + 2);
+    float* part = paged_part(p, HD, it.slot + it.chunk, g) + c16 * (HD + 4);
     float* dst = whole ? p.out + ((int64_t)row * H + g * G + cg) * HD : part;
+    constexpr int TW = DT / NW;  // tiles per wave: consecutive dims
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-        if ((d & (NW - 1)) != wv) continue;
-        f32x4 v = {0, 0, 0, 0};
+    for (int r = 0; r < 4; ++r) {
+        float v[TW];
 #pragma unroll
-        for (int w = 0; w < NW; ++w) v += *reinterpret_cast<const f32x4*>(lds + w * kPart + d * 256 + lane * 4) * wm[w];
+        for (int i = 0; i < TW; ++i) {
+            v[i] = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) dst[DT * (4 * q4 + r) + d] = whole ? (lj == 0.0f ? 0.0f : v[r] * inv_l) : v[r];
+            for (int w = 0; w < NW; ++w) v[i] = fmaf(lds[w * kPart + (TW * wv + i) * 256 + lane * 4 + r], wm[w], v[i]);
+            if (whole) v[i] = lj == 0.0f ? 0.0f : v[i] * inv_l;
+        }
+        float* to = dst + DT * (4 * q4 + r) + TW * wv;
+        if constexpr (TW == 2) *reinterpret_cast<float2*>(to) = float2{v[0], v[1]};
+        else to[0] = v[0];
     }
-    if (!whole && wv == 0 && q4 == 0) {
-        part[HD] = mj;
-        part[HD + 1] = lj;
-    }
+    if (!whole && wv == 0 && q4 == 0) *reinterpret_cast<float2*>(part + HD) = float2{mj, lj};
 }
 
-// joins the chunks of the rows that have several: out = sum e^(m_c - M) acc_c /
-// sum e^(m_c - M) l_c.  Workgroup (row among them, kv head, column); the chunks go
-// round the thread groups of HD threads, whose sums are added in a fixed order.
-constexpr int kCombineThreads = 512;
+// joins the chunks of the rows that have several: out = sum 2^(m_c - M) acc_c /
+// sum 2^(m_c - M) l_c.  Workgroup (row among them, kv head, query head of it); HD /
+// 4 threads hold a head's dims, the chunks go round the groups of threads, each
+// with a running maximum (one pass over the partials), and the groups join in
+// LDS in order.
+constexpr int kCombineThreads = 256;
 template <int HD>
 __global__ __launch_bounds__(kCombineThreads) void k_paged_combine(PagedParams p) {
-    constexpr int NG = kCombineThreads / HD;
-    __shared__ float acc[NG][HD], ssum[NG];
-    const int t = threadIdx.x, d = t % HD, grp = t / HD;
-    const int g = blockIdx.y, c = blockIdx.z, G = p.g;
-    const int C = plan_chunk(p);
+    constexpr int TD = HD / 4, NG = kCombineThreads / TD;
+    __shared__ f32x4 acc[NG][TD];
+    __shared__ float2 ml[NG];
+    const int t = threadIdx.x, d = t % TD, grp = t / TD;
+    const int g = blockIdx.y, G = p.g;
     PlanItem it;
-    if (!plan_find(p, C, blockIdx.x, true, &it)) return;
-    if (c >= it.nr * G) return;
-    const float* src = paged_part(p, HD, it.slot, g) + c * (HD + 2);
-    const int64_t stride = (int64_t)p.n_kv * p.rt * G * (HD + 2);
-    float mx = -INFINITY;
-    for (int i = 0; i < it.chunks; ++i) mx = fmaxf(mx, src[i * stride + HD]);
-    float a = 0.0f, l = 0.0f;
-    for (int i = grp; i < it.chunks; i += NG) {
-        const float m = src[i * stride + HD];
-        const float w = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
-        a = fmaf(src[i * stride + d], w, a);
-        l = fmaf(src[i * stride + HD + 1], w, l);
-    }
-    acc[grp][d] = a;
-    if (d == 0) ssum[grp] = l;
-    __syncthreads();
-    if (grp) return;
+    if (!plan_find<true>(p, blockIdx.x, &it)) return;
+    const int64_t stride = (int64_t)p.n_kv * p.rt * G * (HD + 4);
+    for (int rr = 0; rr < it.nr; ++rr) {
+        const float* src = paged_part(p, HD, it.slot, g) + (rr * G + (int)blockIdx.z) * (HD + 4);
+        f32x4 a = {0, 0, 0, 0};
+        float l = 0.0f, m = -INFINITY;
+#pragma unroll 4
+        for (int i = grp; i < it.chunks; i += NG) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(src + i * stride + 4 * d);
+            const float2 s = *reinterpret_cast<const float2*>(src + i * stride + HD);
+            // chunks and groups without a finite score: their sums are zero, or NaN and stay so
+            const float mn = fmaxf(m, s.x);
+            const float f0 = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            const float f1 = s.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s.x - mn);
+            a = a * f0 + v * f1;
+            l = l * f0 + s.y * f1;
+            m = mn;
+        }
+        acc[grp][d] = a;
+        if (d == 0) ml[grp] = float2{m, l};
+        __syncthreads();
+        if (grp == 0) {
+            float mx = m;
 #pragma unroll
-    for (int i = 1; i < NG; ++i) {
-        a += acc[i][d];
-        l += ssum[i];
+            for (int i = 1; i < NG; ++i) mx = fmaxf(mx, ml[i].x);
+            const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
+            a *= f;
+            l *= f;
+#pragma unroll
+            for (int i = 1; i < NG; ++i) {
+                const float fi = ml[i].x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[i].x - mx);
+                a += acc[i][d] * fi;
+                l = fmaf(ml[i].y, fi, l);
+            }
+            float* o = p.out + ((int64_t)(it.row + rr) * p.n_heads + g * G + (int)blockIdx.z) * HD + 4 * d;
+            *reinterpret_cast<f32x4*>(o) = l == 0.0f ? f32x4{0, 0, 0, 0} : a / l;
+        }
+        __syncthreads();
     }
-    const int rt = c / G;
-    p.out[((int64_t)(it.row + rt) * p.n_heads + g * G + c - rt * G) * HD + d] = l == 0.0f ? 0.0f : a / l;
 }
 
 template <int HD, bool BF16>
 static void launch_paged_t(const PagedParams& p, hipStream_t st) {
-    hipLaunchKernelGGL((k_paged_attend<HD, BF16>), dim3((unsigned)(paged_items(p) * p.n_kv)), dim3(256), 0, st, p);
+    const dim3 grid((unsigned)(paged_items(p) * p.n_kv));
+    if (BF16 && p.T <= p.n_seq) hipLaunchKernelGGL((k_paged_attend<HD, BF16, BF16>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((k_paged_attend<HD, BF16, false>), grid, dim3(256), 0, st, p);
     const int rows = paged_split_rows(p);
     if (rows)
-        hipLaunchKernelGGL((k_paged_combine<HD>), dim3((unsigned)rows, (unsigned)p.n_kv, (unsigned)(p.rt * p.g)),
+        hipLaunchKernelGGL((k_paged_combine<HD>), dim3((unsigned)rows, (unsigned)p.n_kv, (unsigned)p.g),
                            dim3(kCombineThreads), 0, st, p);
 }
 

@@ -5,7 +5,7 @@ import ctypes
 
 import torch
 
-from ._lib import Rules, check, lib
+from ._lib import Rules, check, lib, on
 from .wcomp import _ptr, _stream
 
 
@@ -84,7 +84,7 @@ def adjust(x, out=None, tokens=None, length=None, prompt=None, penalties=None, b
     if T == 0:
         return out
     L = lib()
-    with torch.cuda.device(dev):
+    with on(dev):
         need = L.rv12_logits_workspace_bytes(V, T) if ids is not None else 0
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         check(L.rv12_logits_adjust(ctypes.byref(a), _ptr(x), xs, _ptr(out), ys, V, T, _ptr(ids), _ptr(ws), need,

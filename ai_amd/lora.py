@@ -9,7 +9,7 @@ import ctypes
 
 import torch
 
-from ._lib import Lora, check, lib
+from ._lib import Lora, check, lib, on
 from .wcomp import _ptr, _stream
 
 
@@ -99,7 +99,7 @@ class Adapters:
         if T == 0:
             return out
         L = lib()
-        with torch.cuda.device(dev):
+        with on(dev):
             need = L.rv12_lora_workspace_bytes(self._a.r, K, T)
             if need == 0:
                 raise ValueError("apply: at most 65536 rows")
