@@ -923,7 +923,7 @@ int rv12_logits_adjust(const rv12_rules* rules, const float* x, int64_t x_stride
 // --- low-rank adapters
 size_t rv12_lora_workspace_bytes(int r, int k, int t) {
     if (r < 8 || r % 8 || r > kMaxLoraRank || k < 32 || k % 32 || k > kMaxK || t < 1 || t > 65536) return 0;
-    return (size_t)lora_splits(k, t) * t * (16 * (size_t)lora_rank_blocks(r) + 1) * 4;
+    return (size_t)lora_splits(k) * t * (16 * (size_t)lora_rank_blocks(r) + 1) * 4;
 }
 
 int rv12_lora_apply(const rv12_lora* a, const float* x, const float* y, int64_t y_stride, float* out, int64_t out_stride,
@@ -958,9 +958,8 @@ int rv12_lora_apply(const rv12_lora* a, const float* x, const float* y, int64_t 
     p.R = a->r;
     p.count = a->count;
     p.mode = mode;
-    p.S = lora_splits(a->k, t);
-    p.slots = t <= 64 ? std::min(t, 16) : 2;
-    p.nbw = 4;
+    p.S = lora_splits(a->k);
+    lora_launch(&p);
     p.eps = eps;
     p.h = (float*)ws;
     p.ssq = p.h + (size_t)p.S * t * 16 * lora_rank_blocks(a->r);

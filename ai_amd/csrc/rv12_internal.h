@@ -259,10 +259,18 @@ struct LoraParams {
 constexpr int kMaxLoraRank = 128;
 // blocks of 16 ranks the kernels are built for: 1, 2, 4 or 8
 inline int lora_rank_blocks(int R) { return R <= 16 ? 1 : (R <= 32 ? 2 : (R <= 64 ? 4 : 8)); }
-// K splits: 4 steps of 32 columns per wave while the tiles are few
-inline int lora_splits(int K, int T) {
-    const int tiles = (T + 15) / 16, steps = K / 32;
-    return std::max(1, std::min((steps + 15) / 16, 512 / tiles));
+// K splits of the first pass: 4 steps of 32 columns for each of its 4 waves, at
+// most 16 splits (the second pass adds them 16 lanes at a time)
+inline int lora_splits(int K) { return std::min((K / 32 + 15) / 16, 16); }
+// adapters of a tile side by side (the grid takes that many whether they are there
+// or not): all 16 while the tiles are few.  Blocks per wave of the second pass: as
+// many as leave 256 workgroups, which prepare the tile's h each (13 adapters, rank
+// 32, 6144 rows: 6.0 us with 4 blocks, 6.4 with 2 or 8, 10.1 with one)
+inline void lora_launch(LoraParams* p) {
+    const int tiles = (p->T + 15) / 16, nblk = (p->N + 15) / 16;
+    p->slots = std::min(std::min(p->T, 16), std::max(1, 64 / tiles));
+    p->nbw = 16;
+    while (p->nbw > 1 && (int64_t)((nblk + 4 * p->nbw - 1) / (4 * p->nbw)) * tiles * p->slots < 256) p->nbw /= 2;
 }
 void launch_lora(const LoraParams& p, bool vec, hipStream_t st);
 

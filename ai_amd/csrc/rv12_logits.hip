@@ -23,7 +23,11 @@ namespace rv12 {
 // the generated ones
 constexpr uint32_t kSeen = 0x80000000u;
 
+// VEC: the rows of x and y at 16-byte addresses, V a multiple of 4 (a slice is one)
+template <bool VEC>
 __global__ __launch_bounds__(kAdjustThreads) void k_adjust(AdjustParams p) {
+    constexpr int W = VEC ? 4 : 1;  // ids of a thread at once
+    constexpr int U = VEC ? 4 : 8;  // loads of a thread in flight
     extern __shared__ uint32_t cnt[];  // [slice], then the bias entries' places [slice]
     const int r = blockIdx.y, t = threadIdx.x, lane = t & 63;
     const int64_t n0 = (int64_t)blockIdx.x * p.slice;
@@ -31,13 +35,15 @@ __global__ __launch_bounds__(kAdjustThreads) void k_adjust(AdjustParams p) {
     int* bias_at = reinterpret_cast<int*>(cnt + p.slice);
     const int L = p.tokens ? (int)min(max(p.length[r], 0), p.max_tokens) : 0;
     const int made = p.prompt ? max(p.prompt[r], 0) : 0;
-    for (int i = t; i < ns; i += kAdjustThreads) {
-        cnt[i] = 0;
-        if (p.n_bias) bias_at[i] = 0;
-    }
-    __syncthreads();
-    if (L) {
+    const bool counts = L > 0, biased = p.n_bias > 0;
+    if (counts || biased) {
+        for (int i = t; i < ns; i += kAdjustThreads) {
+            cnt[i] = 0;
+            if (biased) bias_at[i] = 0;
+        }
+        __syncthreads();
         const int64_t* tok = p.tokens + (int64_t)r * p.tokens_stride;
+#pragma unroll 8
         for (int i = t; i < L; i += kAdjustThreads) {
             const int64_t n = tok[i] - n0;
             if (n >= 0 && n < ns) {
@@ -45,15 +51,13 @@ __global__ __launch_bounds__(kAdjustThreads) void k_adjust(AdjustParams p) {
                 if (i >= made) atomicAdd(&cnt[n], 1u);
             }
         }
-    }
-    if (p.n_bias) {
         const int64_t* id = p.bias_ids + (int64_t)r * p.bias_stride;
         for (int i = t; i < p.n_bias; i += kAdjustThreads) {
             const int64_t n = id[i] - n0;
             if (n >= 0 && n < ns) atomicMax(&bias_at[n], i + 1);  // the last entry of an id counts
         }
+        __syncthreads();
     }
-    __syncthreads();
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     if (p.penalties) {
         rep = p.penalties[3 * r];
@@ -62,26 +66,54 @@ __global__ __launch_bounds__(kAdjustThreads) void k_adjust(AdjustParams p) {
     }
     const float* x = p.x + (int64_t)r * p.x_stride + n0;
     float* y = p.y + (int64_t)r * p.y_stride + n0;
-    const uint32_t* mask = p.mask ? p.mask + (int64_t)r * p.mask_stride : nullptr;
+    // (a slice starts at a multiple of 32 ids)
+    const uint32_t* mask = p.mask ? p.mask + (int64_t)r * p.mask_stride + (n0 >> 5) : nullptr;
     const float* bias = p.bias + (int64_t)r * p.bias_stride;
     float bv = -INFINITY;
     int bi = 0x7FFFFFFF;
-    for (int i = t; i < ns; i += kAdjustThreads) {
-        const int64_t n = n0 + i;
-        const bool ok = !mask || (mask[n >> 5] >> (n & 31) & 1u);
-        float v = x[i];
-        const uint32_t c = cnt[i];
-        if (c) {
-            v = v > 0.0f ? v / rep : v * rep;
-            const uint32_t k = c & ~kSeen;
-            if (k) v -= freq * (float)k + pres;
+    for (int i0 = t * W; i0 < ns; i0 += U * kAdjustThreads * W) {
+        float v[U][W];
+        uint32_t ok[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * kAdjustThreads * W;
+            ok[u] = 0;
+            if (i >= ns) break;
+            if constexpr (VEC) {
+                const f32x4 q = *reinterpret_cast<const f32x4*>(x + i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[u][e] = q[e];
+            } else {
+                v[u][0] = x[i];
+            }
+            ok[u] = mask ? mask[i >> 5] >> (i & 31) : 0xFu;
         }
-        if (p.n_bias && bias_at[i]) v += bias[bias_at[i] - 1];
-        if (!ok) v = -INFINITY;
-        y[i] = v;
-        if (ok && pick_beats(v, (int)n, bv, bi)) {
-            bv = v;
-            bi = (int)n;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * kAdjustThreads * W;
+            if (i >= ns) break;
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                float f = v[u][e];
+                if (counts) {
+                    const uint32_t c = cnt[i + e];
+                    if (c) {
+                        f = f > 0.0f ? f / rep : f * rep;
+                        const uint32_t k = c & ~kSeen;
+                        if (k) f -= freq * (float)k + pres;
+                    }
+                }
+                if (biased && bias_at[i + e]) f += bias[bias_at[i + e] - 1];
+                const bool may = ok[u] >> e & 1u;
+                f = may ? f : -INFINITY;
+                v[u][e] = f;
+                if (may && pick_beats(f, (int)n0 + i + e, bv, bi)) {
+                    bv = f;
+                    bi = (int)n0 + i + e;
+                }
+            }
+            if constexpr (VEC) *reinterpret_cast<f32x4*>(y + i) = f32x4{v[u][0], v[u][1], v[u][2], v[u][3]};
+            else y[i] = v[u][0];
         }
     }
     if (!p.pv) return;
@@ -140,8 +172,12 @@ __global__ __launch_bounds__(64) void k_adjust_pick(const float* pv, const int32
 void launch_adjust(const AdjustParams& pa, int T, int64_t* ids, hipStream_t st) {
     AdjustParams p = pa;
     const int ns = (int)((p.V + p.slice - 1) / p.slice);
-    hipLaunchKernelGGL(k_adjust, dim3((unsigned)ns, (unsigned)T), dim3(kAdjustThreads),
-                       (size_t)p.slice * (p.n_bias ? 8 : 4), st, p);
+    const bool vec = p.V % 4 == 0 && (((uintptr_t)p.x | (uintptr_t)p.y) & 15u) == 0 &&
+                     (T == 1 || (p.x_stride % 4 == 0 && p.y_stride % 4 == 0));
+    const dim3 grid((unsigned)ns, (unsigned)T);
+    const size_t lds = (size_t)p.slice * (p.n_bias ? 8 : 4);
+    if (vec) hipLaunchKernelGGL((k_adjust<true>), grid, dim3(kAdjustThreads), lds, st, p);
+    else hipLaunchKernelGGL((k_adjust<false>), grid, dim3(kAdjustThreads), lds, st, p);
     if (ids) hipLaunchKernelGGL(k_adjust_pick, dim3((unsigned)T), dim3(64), 0, st, p.pv, p.pi, ns, ids);
 }
 

@@ -31,23 +31,30 @@ __device__ __forceinline__ bool tile_slot(const LoraParams& p, int t0, int s, in
         a = p.idx[t0 + c];
         if (a < 0 || a >= p.count) a = -1;
     }
-    bool lead = a != -2;
-    for (int j = 0; j < 15; ++j) lead = lead && !(j < c && __builtin_amdgcn_readlane(a, j) == a);
-    uint64_t m = __ballot(lead) & 0xFFFFull;
-    for (int j = 0; j < s && m; ++j) m &= m - 1;
-    if (!m) return false;
-    *id = __builtin_amdgcn_readlane(a, __builtin_ctzll(m));
-    *mine = a == *id;
-    return true;
+    uint64_t left = __ballot(a != -2) & 0xFFFFull;
+    for (; left; --s) {
+        const int first = __builtin_amdgcn_readlane(a, __builtin_ctzll(left));
+        if (s == 0) {
+            *id = first;
+            *mine = a == first;
+            return true;
+        }
+        left &= ~__ballot(a == first);
+    }
+    return false;
 }
 
 // 1. h[split][t][j] = sum over the split's columns of A[j] x'[t] (before the
 // RMSNorm's factor), ssq[split][t] = their sum of squares (scaled).  Four waves
-// share the split's steps of 32 columns and join in LDS.
-template <int RB>  // blocks of 16 ranks
+// share the split's steps of 32 columns and join in LDS.  The splits spread the
+// adapter's weights over the CUs (a CU reads them from HBM at some 20 GB/s: 16
+// rows of 13 adapters, rank 32, 4096 columns, take 6.7 us in 8 splits of 4 waves,
+// 17.5 in one of 16).
+template <int RB, bool MODE2>  // blocks of 16 ranks; x' = silu(g) u
 __global__ __launch_bounds__(256) void k_lora_down(LoraParams p) {
-    __shared__ f32x4 acc_lds[4][RB][64];
-    __shared__ float ssq_lds[4][16];
+    constexpr int NW = 4;
+    __shared__ f32x4 acc_lds[NW][RB][64];
+    __shared__ float ssq_lds[NW][16];
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q4 = lane >> 4, c16 = lane & 15;
@@ -61,29 +68,36 @@ __global__ __launch_bounds__(256) void k_lora_down(LoraParams p) {
         const int nb = (rank + 15) / 16;
         const int steps = p.K / 32;
         const int s0 = (int)((int64_t)sp * steps / p.S), s1 = (int)((int64_t)(sp + 1) * steps / p.S);
-        const float* x = p.x + (int64_t)(t0 + c16) * (p.mode == 2 ? 2 * (int64_t)p.K : p.K) + 8 * q4;
+        const float* x = p.x + (int64_t)(t0 + c16) * (MODE2 ? 2 : 1) * p.K + 8 * q4;
         const uint16_t* A = p.A + (int64_t)id * p.R * p.K + 8 * q4;
         f32x4 acc[RB];
 #pragma unroll
         for (int b = 0; b < RB; ++b) acc[b] = f32x4{0, 0, 0, 0};
         float ss = 0.0f;
-        for (int s = s0 + wv; s < s1; s += 4) {
-            float v[8];
+        // the loads of a step, one step ahead of its products
+        f32x4 xg[2], xu[2];
+        u32x4 w, av[RB];
+        auto load = [&](int s) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                f32x4 g = {0, 0, 0, 0};
-                if (mine) g = *reinterpret_cast<const f32x4*>(x + 32 * s + 4 * c);
-                if (p.mode == 2) {
-                    f32x4 u = {0, 0, 0, 0};
-                    if (mine) u = *reinterpret_cast<const f32x4*>(x + p.K + 32 * s + 4 * c);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) g[e] = silu_mul(g[e], u[e]);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * c + e] = g[e];
+                xg[c] = xu[c] = f32x4{0, 0, 0, 0};
+                if (mine) xg[c] = *reinterpret_cast<const f32x4*>(x + 32 * s + 4 * c);
+                if (mine && MODE2) xu[c] = *reinterpret_cast<const f32x4*>(x + p.K + 32 * s + 4 * c);
             }
-            if (p.lnw) {
-                const u32x4 w = *reinterpret_cast<const u32x4*>(p.lnw + 32 * s + 8 * q4);
+            if (!MODE2 && p.lnw) w = *reinterpret_cast<const u32x4*>(p.lnw + 32 * s + 8 * q4);
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+                if (b < nb) av[b] = *reinterpret_cast<const u32x4*>(A + (int64_t)min(16 * b + c16, p.R - 1) * p.K + 32 * s);
+        };
+        if (s0 + wv < s1) load(s0 + wv);
+        for (int s = s0 + wv; s < s1; s += NW) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = xg[e >> 2][e & 3];
+                if constexpr (MODE2) v[e] = silu_mul(v[e], xu[e >> 2][e & 3]);
+            }
+            if (!MODE2 && p.lnw) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float sv = v[e] * kSsqScale;
@@ -91,103 +105,172 @@ __global__ __launch_bounds__(256) void k_lora_down(LoraParams p) {
                     v[e] *= (e & 1) ? hi_f(w[e >> 1]) : lo_f(w[e >> 1]);
                 }
             }
+            u32x4 a[RB];
+#pragma unroll
+            for (int b = 0; b < RB; ++b) a[b] = av[b];
+            if (s + NW < s1) load(s + NW);
             u32x4 h, m, l;
             split3(v, h, m, l);
 #pragma unroll
             for (int b = 0; b < RB; ++b) {
                 if (b >= nb) break;
-                const int j = min(16 * b + c16, p.R - 1);
-                const u32x4 a = *reinterpret_cast<const u32x4*>(A + (int64_t)j * p.K + 32 * s);
-                acc[b] = mfma(a, h, acc[b]);
-                acc[b] = mfma(a, m, acc[b]);
-                acc[b] = mfma(a, l, acc[b]);
+                acc[b] = mfma(a[b], h, acc[b]);
+                acc[b] = mfma(a[b], m, acc[b]);
+                acc[b] = mfma(a[b], l, acc[b]);
             }
         }
         ss += __shfl_xor(ss, 16);
         ss += __shfl_xor(ss, 32);
+        if (q4 == 0) ssq_lds[wv][c16] = ss;
 #pragma unroll
         for (int b = 0; b < RB; ++b) acc_lds[wv][b][lane] = acc[b];
-        if (q4 == 0) ssq_lds[wv][c16] = ss;
         __syncthreads();
         float* h = p.h + ((int64_t)sp * p.T + t0 + c16) * (16 * RB);
-        for (int b = wv; b < nb; b += 4) {
+        for (int b = wv; b < nb; b += NW) {
             f32x4 v = acc_lds[0][b][lane];
-            for (int w = 1; w < 4; ++w) v += acc_lds[w][b][lane];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) v += acc_lds[w][b][lane];
             if (mine) *reinterpret_cast<f32x4*>(h + 16 * b + 4 * q4) = v;
         }
-        if (wv == 0 && q4 == 0 && mine && p.lnw)
-            p.ssq[(int64_t)sp * p.T + t0 + c16] = (ssq_lds[0][c16] + ssq_lds[1][c16]) + (ssq_lds[2][c16] + ssq_lds[3][c16]);
+        if (wv == 0 && q4 == 0 && mine && !MODE2 && p.lnw) {
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) v += ssq_lds[w][c16];
+            p.ssq[(int64_t)sp * p.T + t0 + c16] = v;
+        }
         __syncthreads();
     }
 }
 
 // 2. out[t][n] = y[t][n] + sum_j B[n][j] (factor h[t][j]), factor = scale times
-// the RMSNorm's.  A wave has the tile's h in registers and takes blocks of 16
-// output rows.
+// the RMSNorm's.  The workgroup adds the splits' h (every thread one part of it, all
+// loads at once) and leaves it in LDS as the products' operand; then a wave takes
+// p.nbw consecutive blocks of 16 output rows, UB at a time, the weights and y of
+// the next UB loaded ahead of the products and stores of these.
 template <int RB, bool VEC>  // VEC: y and out rows at 16-byte addresses, N % 4 == 0
 __global__ __launch_bounds__(256) void k_lora_up(LoraParams p) {
     constexpr int RS = (RB + 1) / 2;  // steps of 32 ranks
+    constexpr int UB = RB == 8 ? 2 : 4;
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q4 = lane >> 4, c16 = lane & 15;
     const int t0 = blockIdx.y * 16, t = t0 + c16;
-    const int nb0 = blockIdx.x * p.nbw * 4 + wv;  // first block of 16 rows, every fourth from there
-    const int nblk = (p.N + 15) / 16;
-    if (nb0 >= nblk) return;
+    const int nb0 = (blockIdx.x * 4 + wv) * p.nbw, nb1 = min(nb0 + p.nbw, (p.N + 15) / 16);
+    constexpr int HE = 64 * RB;             // float4 parts of the tile's h
+    constexpr int GR = HE < 256 ? 256 / HE : 1;  // thread groups that share the splits
+    constexpr int PE = HE > 256 ? HE / 256 : 1;  // parts of a thread
+    __shared__ f32x4 part[GR][HE];
+    __shared__ u32x4 hl[RS][3][64];
+    __shared__ float factor[16];
     for (int slot = blockIdx.z;; slot += gridDim.z) {
         int id;
         bool mine;
         if (!tile_slot(p, t0, slot, &id, &mine)) return;
         if (id < 0 && p.y == p.out) continue;
         const int rank = id < 0 ? 0 : (p.ranks ? min(max(p.ranks[id], 0), p.R) : p.R);
+        const uint16_t* B = p.B + (int64_t)max(id, 0) * p.N * p.R + 8 * q4;
+        u32x4 bv[UB][RS];
+        f32x4 yv[UB];
+        auto load = [&](int nb) {
+#pragma unroll
+            for (int u = 0; u < UB; ++u) {
+                if (nb + u >= nb1) break;
+                const int n = min(16 * (nb + u) + c16, p.N - 1), no = 16 * (nb + u) + 4 * q4;
+#pragma unroll
+                for (int s = 0; s < RS; ++s) {
+                    bv[u][s] = u32x4{0, 0, 0, 0};
+                    if (32 * s < rank && 32 * s + 8 * q4 < p.R)
+                        bv[u][s] = *reinterpret_cast<const u32x4*>(B + (int64_t)n * p.R + 32 * s);
+                }
+                const float* y = p.y + (int64_t)t * p.y_stride + no;
+                if constexpr (VEC) {
+                    if (mine && no < p.N) yv[u] = *reinterpret_cast<const f32x4*>(y);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (mine && no + e < p.N) yv[u][e] = y[e];
+                }
+            }
+        };
+        load(nb0);
         u32x4 hp[RS][3];
-        if (rank > 0) {
-            float f = mine ? p.scale[id] : 0.0f;
-            if (p.lnw) {
-                float ss = 0.0f;
-                for (int s = 0; s < p.S; ++s) ss += mine ? p.ssq[(int64_t)s * p.T + t] : 0.0f;
-                f *= rms_scale(ss, p.K, p.eps);
+        if (rank > 0) {  // (the same for the whole workgroup)
+            const int tid = threadIdx.x;
+            {
+                // the factor of row tid / 16: its 16 lanes take a split each
+                const int r = min(t0 + (tid >> 4), p.T - 1), k = tid & 15;
+                float ss = p.lnw && k < p.S ? p.ssq[(int64_t)k * p.T + r] : 0.0f;
+                ss += dpp<kDppXor1>(ss);
+                ss += dpp<kDppXor2>(ss);
+                ss += dpp<kDppHalfMirror>(ss);
+                ss += dpp<kDppMirror>(ss);
+                if (k == 0) factor[tid >> 4] = p.scale[id] * (p.lnw ? rms_scale(ss, p.K, p.eps) : 1.0f);
             }
 #pragma unroll
-            for (int s = 0; s < RS; ++s) {
+            for (int i = 0; i < PE; ++i) {
+                const int e = tid % HE + 256 * i, r = e / (4 * RB), grp = tid / HE;
+                // (rows past the last are clamped and what is another adapter's, or
+                // past the rank, dropped below: no condition on the loads)
+                const float* h = p.h + (int64_t)min(t0 + r, p.T - 1) * (16 * RB) + 4 * (e % (4 * RB));
+                f32x4 a = {0, 0, 0, 0};
+#pragma unroll 4
+                for (int k = grp; k < p.S; k += GR) a += *reinterpret_cast<const f32x4*>(h + (int64_t)k * p.T * (16 * RB));
+                part[grp][e] = a;
+            }
+            __syncthreads();
+            for (int s = wv; s < RS; s += 4) {
                 float v[8];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    f32x4 a = {0, 0, 0, 0};
-                    const int j = 32 * s + 8 * q4 + 4 * c;
-                    if (mine && j < rank)
-                        for (int k = 0; k < p.S; ++k)
-                            a += *reinterpret_cast<const f32x4*>(p.h + ((int64_t)k * p.T + t) * (16 * RB) + j);
+                for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+                if (32 * s + 8 * q4 < 16 * RB) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[4 * c + e] = j + e < rank ? a[e] * f : 0.0f;
+                    for (int c = 0; c < 2; ++c) {
+                        f32x4 a = part[0][c16 * 4 * RB + 8 * s + 2 * q4 + c];
+#pragma unroll
+                        for (int i = 1; i < GR; ++i) a += part[i][c16 * 4 * RB + 8 * s + 2 * q4 + c];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            v[4 * c + e] = mine && 32 * s + 8 * q4 + 4 * c + e < rank ? a[e] * factor[c16] : 0.0f;
+                    }
                 }
-                split3(v, hp[s][0], hp[s][1], hp[s][2]);
+                u32x4 hi, mid, lo;
+                split3(v, hi, mid, lo);
+                hl[s][0][lane] = hi;
+                hl[s][1][lane] = mid;
+                hl[s][2][lane] = lo;
             }
+            __syncthreads();
+#pragma unroll
+            for (int s = 0; s < RS; ++s)
+#pragma unroll
+                for (int c = 0; c < 3; ++c) hp[s][c] = hl[s][c][lane];
         }
-        const uint16_t* B = p.B + (int64_t)max(id, 0) * p.N * p.R + 8 * q4;
-        for (int i = 0; i < p.nbw; ++i) {
-            const int nb = nb0 + 4 * i;
-            if (nb >= nblk) break;
-            f32x4 acc = {0, 0, 0, 0};
-            const int n = min(16 * nb + c16, p.N - 1);
+        for (int nb = nb0; nb < nb1; nb += UB) {
+            f32x4 acc[UB];
 #pragma unroll
-            for (int s = 0; s < RS; ++s) {
-                if (32 * s >= rank) break;
-                u32x4 b = {0, 0, 0, 0};
-                if (32 * s + 8 * q4 < p.R) b = *reinterpret_cast<const u32x4*>(B + (int64_t)n * p.R + 32 * s);
+            for (int u = 0; u < UB; ++u) {
+                acc[u] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int c = 0; c < 3; ++c) acc = mfma(b, hp[s][c], acc);
+                for (int s = 0; s < RS; ++s) {
+                    if (32 * s >= rank) break;
+#pragma unroll
+                    for (int c = 0; c < 3; ++c) acc[u] = mfma(bv[u][s], hp[s][c], acc[u]);
+                }
+                acc[u] += yv[u];
             }
-            if (!mine) continue;
-            const int no = 16 * nb + 4 * q4;
-            const float* y = p.y + (int64_t)t * p.y_stride + no;
-            float* o = p.out + (int64_t)t * p.out_stride + no;
-            if constexpr (VEC) {
-                if (no < p.N) *reinterpret_cast<f32x4*>(o) = *reinterpret_cast<const f32x4*>(y) + acc;
-            } else {
+            if (nb + UB < nb1) load(nb + UB);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (no + e < p.N) o[e] = y[e] + acc[e];
+            for (int u = 0; u < UB; ++u) {
+                const int no = 16 * (nb + u) + 4 * q4;
+                if (!mine || nb + u >= nb1) continue;
+                float* o = p.out + (int64_t)t * p.out_stride + no;
+                if constexpr (VEC) {
+                    if (no < p.N) *reinterpret_cast<f32x4*>(o) = acc[u];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (no + e < p.N) o[e] = acc[u][e];
+                }
             }
         }
     }
@@ -196,7 +279,9 @@ __global__ __launch_bounds__(256) void k_lora_up(LoraParams p) {
 template <int RB>
 static void launch_lora_t(const LoraParams& p, bool vec, hipStream_t st) {
     const unsigned tiles = (unsigned)((p.T + 15) / 16), nblk = (unsigned)((p.N + 15) / 16);
-    hipLaunchKernelGGL((k_lora_down<RB>), dim3((unsigned)p.S, tiles, (unsigned)p.slots), dim3(256), 0, st, p);
+    const dim3 d((unsigned)p.S, tiles, (unsigned)p.slots);
+    if (p.mode == 2) hipLaunchKernelGGL((k_lora_down<RB, true>), d, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((k_lora_down<RB, false>), d, dim3(256), 0, st, p);
     const dim3 g((nblk + 4 * p.nbw - 1) / (4 * p.nbw), tiles, (unsigned)p.slots);
     if (vec) hipLaunchKernelGGL((k_lora_up<RB, true>), g, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((k_lora_up<RB, false>), g, dim3(256), 0, st, p);
