@@ -19,42 +19,85 @@
 
 namespace rv12 {
 
-// counts of a slice: bit 31 set once the id is among the row's tokens, below it
-// the generated ones
-constexpr uint32_t kSeen = 0x80000000u;
+// counts of a slice: bit 31 set once the id is among the row's tokens, bit 30 once
+// it has a bias, below them the generated tokens
+constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u;
+constexpr int kNoId = 0x7FFFFFFF;
 
-// VEC: the rows of x and y at 16-byte addresses, V a multiple of 4 (a slice is one)
-template <bool VEC>
+// four floats at a 4-byte address (one 16-byte access all the same): rows of an odd
+// vocabulary start anywhere
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
 __global__ __launch_bounds__(kAdjustThreads) void k_adjust(AdjustParams p) {
-    constexpr int W = VEC ? 4 : 1;  // ids of a thread at once
-    constexpr int U = VEC ? 4 : 8;  // loads of a thread in flight
-    extern __shared__ uint32_t cnt[];  // [slice], then the bias entries' places [slice]
+    constexpr int U = 4;               // 16-byte loads of a thread in flight
+    constexpr int TB = 8;              // tokens of a thread in flight
+    constexpr int kStep = 4 * kAdjustThreads;
+    extern __shared__ u32x4 lds[];     // counts [slice], then the bias entries' places [slice]
+    uint32_t* cnt = reinterpret_cast<uint32_t*>(lds);
+    int* bias_at = reinterpret_cast<int*>(cnt + p.slice);
     const int r = blockIdx.y, t = threadIdx.x, lane = t & 63;
     const int64_t n0 = (int64_t)blockIdx.x * p.slice;
     const int ns = (int)min((int64_t)p.slice, p.V - n0);
-    int* bias_at = reinterpret_cast<int*>(cnt + p.slice);
     const int L = p.tokens ? (int)min(max(p.length[r], 0), p.max_tokens) : 0;
     const int made = p.prompt ? max(p.prompt[r], 0) : 0;
-    const bool counts = L > 0, biased = p.n_bias > 0;
-    if (counts || biased) {
-        for (int i = t; i < ns; i += kAdjustThreads) {
-            cnt[i] = 0;
-            if (biased) bias_at[i] = 0;
+    const bool any = L > 0 || p.n_bias > 0;
+    const float* x = p.x + (int64_t)r * p.x_stride + n0;
+    float* y = p.y + (int64_t)r * p.y_stride + n0;
+    // (a slice starts at a multiple of 32 ids)
+    const uint32_t* mask = p.mask ? p.mask + (int64_t)r * p.mask_stride + (n0 >> 5) : nullptr;
+    const float* bias = p.bias + (int64_t)r * p.bias_stride;
+    f32x4 v[U];
+    uint32_t ok[U];
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * kStep;
+            if (i >= ns) break;
+            if (i + 4 <= ns) {
+                v[u] = *reinterpret_cast<const f32x4u*>(x + i);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[u][e] = i + e < ns ? x[i + e] : 0.0f;
+            }
+            // past the row's end no id is allowed
+            ok[u] = (mask ? mask[i >> 5] >> (i & 31) : 0xFu) & (i + 4 <= ns ? 0xFu : (1u << (ns - i)) - 1u);
+        }
+    };
+    load(4 * t);  // the slice's first logits are on their way while its tokens are counted
+    if (any) {
+        const int64_t* tok = p.tokens + (int64_t)r * p.tokens_stride;
+        const int64_t* id = p.bias_ids + (int64_t)r * p.bias_stride;
+        int64_t n[TB];
+#pragma unroll
+        for (int u = 0; u < TB; ++u) n[u] = L ? tok[min(t + u * kAdjustThreads, L - 1)] : 0;
+        int64_t nb = t < p.n_bias ? id[t] : -1;
+        for (int i = t; i < p.slice / 4; i += kAdjustThreads) {
+            lds[i] = u32x4{0, 0, 0, 0};
+            if (p.n_bias) lds[p.slice / 4 + i] = u32x4{0, 0, 0, 0};
         }
         __syncthreads();
-        const int64_t* tok = p.tokens + (int64_t)r * p.tokens_stride;
-#pragma unroll 8
-        for (int i = t; i < L; i += kAdjustThreads) {
-            const int64_t n = tok[i] - n0;
-            if (n >= 0 && n < ns) {
-                atomicOr(&cnt[n], kSeen);
-                if (i >= made) atomicAdd(&cnt[n], 1u);
+        for (int i0 = t; i0 < L; i0 += TB * kAdjustThreads) {
+#pragma unroll
+            for (int u = 0; u < TB; ++u) {
+                const int i = i0 + u * kAdjustThreads;
+                const int64_t k = n[u] - n0;
+                if (i < L && k >= 0 && k < ns) {
+                    atomicOr(&cnt[k], kSeen);
+                    if (i >= made) atomicAdd(&cnt[k], 1u);
+                }
+            }
+            if (i0 + TB * kAdjustThreads < L) {
+#pragma unroll
+                for (int u = 0; u < TB; ++u) n[u] = tok[min(i0 + (TB + u) * kAdjustThreads, L - 1)];
             }
         }
-        const int64_t* id = p.bias_ids + (int64_t)r * p.bias_stride;
         for (int i = t; i < p.n_bias; i += kAdjustThreads) {
-            const int64_t n = id[i] - n0;
-            if (n >= 0 && n < ns) atomicMax(&bias_at[n], i + 1);  // the last entry of an id counts
+            const int64_t k = nb - n0;
+            if (k >= 0 && k < ns) {
+                atomicOr(&cnt[k], kBiased);
+                atomicMax(&bias_at[k], i);  // the last entry of an id counts
+            }
+            if (i + kAdjustThreads < p.n_bias) nb = id[i + kAdjustThreads];
         }
         __syncthreads();
     }
@@ -64,56 +107,47 @@ __global__ __launch_bounds__(kAdjustThreads) void k_adjust(AdjustParams p) {
         freq = p.penalties[3 * r + 1];
         pres = p.penalties[3 * r + 2];
     }
-    const float* x = p.x + (int64_t)r * p.x_stride + n0;
-    float* y = p.y + (int64_t)r * p.y_stride + n0;
-    // (a slice starts at a multiple of 32 ids)
-    const uint32_t* mask = p.mask ? p.mask + (int64_t)r * p.mask_stride + (n0 >> 5) : nullptr;
-    const float* bias = p.bias + (int64_t)r * p.bias_stride;
     float bv = -INFINITY;
-    int bi = 0x7FFFFFFF;
-    for (int i0 = t * W; i0 < ns; i0 += U * kAdjustThreads * W) {
-        float v[U][W];
-        uint32_t ok[U];
+    int bi = kNoId;
+    for (int i0 = 4 * t; i0 < ns; i0 += U * kStep) {
+        if (i0 != 4 * t) load(i0);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * kAdjustThreads * W;
-            ok[u] = 0;
+            const int i = i0 + u * kStep;
             if (i >= ns) break;
-            if constexpr (VEC) {
-                const f32x4 q = *reinterpret_cast<const f32x4*>(x + i);
+            u32x4 c = {0, 0, 0, 0};
+            if (any) c = lds[i >> 2];
+            if (c[0] | c[1] | c[2] | c[3]) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[u][e] = q[e];
-            } else {
-                v[u][0] = x[i];
-            }
-            ok[u] = mask ? mask[i >> 5] >> (i & 31) : 0xFu;
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * kAdjustThreads * W;
-            if (i >= ns) break;
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                float f = v[u][e];
-                if (counts) {
-                    const uint32_t c = cnt[i + e];
-                    if (c) {
+                for (int e = 0; e < 4; ++e) {
+                    float f = v[u][e];
+                    if (c[e] & kSeen) {
                         f = f > 0.0f ? f / rep : f * rep;
-                        const uint32_t k = c & ~kSeen;
+                        const uint32_t k = c[e] & ~(kSeen | kBiased);
                         if (k) f -= freq * (float)k + pres;
                     }
+                    if (c[e] & kBiased) f += bias[bias_at[i + e]];
+                    v[u][e] = f;
                 }
-                if (biased && bias_at[i + e]) f += bias[bias_at[i + e] - 1];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
                 const bool may = ok[u] >> e & 1u;
-                f = may ? f : -INFINITY;
+                const float f = may ? v[u][e] : -INFINITY;
                 v[u][e] = f;
-                if (may && pick_beats(f, (int)n0 + i + e, bv, bi)) {
+                // (the thread's ids ascend: the first, a larger one, the first NaN)
+                if (may && (bi == kNoId || (!(f <= bv) && bv == bv))) {
                     bv = f;
                     bi = (int)n0 + i + e;
                 }
             }
-            if constexpr (VEC) *reinterpret_cast<f32x4*>(y + i) = f32x4{v[u][0], v[u][1], v[u][2], v[u][3]};
-            else y[i] = v[u][0];
+            if (i + 4 <= ns) {
+                *reinterpret_cast<f32x4u*>(y + i) = v[u];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i + e < ns) y[i + e] = v[u][e];
+            }
         }
     }
     if (!p.pv) return;
@@ -148,7 +182,7 @@ __global__ __launch_bounds__(kAdjustThreads) void k_adjust(AdjustParams p) {
 __global__ __launch_bounds__(64) void k_adjust_pick(const float* pv, const int32_t* pi, int n, int64_t* ids) {
     const int r = blockIdx.x, lane = threadIdx.x;
     float bv = -INFINITY;
-    int bi = 0x7FFFFFFF;
+    int bi = kNoId;
     for (int i = lane; i < n; i += 64) {
         const float v = pv[(int64_t)r * n + i];
         const int k = pi[(int64_t)r * n + i];
@@ -166,18 +200,14 @@ __global__ __launch_bounds__(64) void k_adjust_pick(const float* pv, const int32
             bi = oi;
         }
     }
-    if (lane == 0) ids[r] = bi == 0x7FFFFFFF ? -1 : bi;
+    if (lane == 0) ids[r] = bi == kNoId ? -1 : bi;
 }
 
 void launch_adjust(const AdjustParams& pa, int T, int64_t* ids, hipStream_t st) {
     AdjustParams p = pa;
     const int ns = (int)((p.V + p.slice - 1) / p.slice);
-    const bool vec = p.V % 4 == 0 && (((uintptr_t)p.x | (uintptr_t)p.y) & 15u) == 0 &&
-                     (T == 1 || (p.x_stride % 4 == 0 && p.y_stride % 4 == 0));
-    const dim3 grid((unsigned)ns, (unsigned)T);
-    const size_t lds = (size_t)p.slice * (p.n_bias ? 8 : 4);
-    if (vec) hipLaunchKernelGGL((k_adjust<true>), grid, dim3(kAdjustThreads), lds, st, p);
-    else hipLaunchKernelGGL((k_adjust<false>), grid, dim3(kAdjustThreads), lds, st, p);
+    hipLaunchKernelGGL(k_adjust, dim3((unsigned)ns, (unsigned)T), dim3(kAdjustThreads),
+                       (size_t)p.slice * (p.n_bias ? 8 : 4), st, p);
     if (ids) hipLaunchKernelGGL(k_adjust_pick, dim3((unsigned)T), dim3(64), 0, st, p.pv, p.pi, ns, ids);
 }
 
