@@ -10,16 +10,19 @@ from .wcomp import _ptr, _stream
 
 
 def _rows(t, name, dtype, T, n, dev):
-    """[T, n] (n None: any) with contiguous rows, any stride between them."""
-    if not torch.is_tensor(t) or t.dtype != dtype or t.dim() != 2 or t.device != dev:
+    """Stride between the rows of t: [T, n] (n None: any), each contiguous."""
+    if not torch.is_tensor(t) or t.dtype != dtype or t.dim() != 2 or t.get_device() != dev:
         raise ValueError(f"adjust: {name} must be a 2-D {dtype} tensor on the device of x")
-    if t.shape[0] != T or (n is not None and t.shape[1] != n) or (t.shape[1] > 1 and t.stride(1) != 1):
+    rows, m = t.shape
+    stride, one = t.stride()
+    if rows != T or (n is not None and m != n) or (one != 1 and m > 1):
         raise ValueError(f"adjust: {name} must have {T} rows" + ("" if n is None else f" of {n}") + ", contiguous each")
-    return t.stride(0) if T > 1 else t.shape[1]
+    return stride if T > 1 else m
 
 
 def _vector(t, name, dtype, T, dev):
-    if not torch.is_tensor(t) or t.dtype != dtype or tuple(t.shape) != (T,) or not t.is_contiguous() or t.device != dev:
+    if (not torch.is_tensor(t) or t.dtype != dtype or t.dim() != 1 or t.numel() != T or not t.is_contiguous()
+            or t.get_device() != dev):
         raise ValueError(f"adjust: {name} must be a contiguous {dtype} vector of {T} entries on the device of x")
 
 
@@ -51,42 +54,48 @@ def adjust(x, out=None, tokens=None, length=None, prompt=None, penalties=None, b
         raise ValueError("adjust: x must be a tensor on the GPU")
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError("adjust: x must be [T, V]")
-    (T, V), dev = x.shape, x.device
-    out = x if out is None else out
-    xs, ys = _rows(x, "x", torch.float32, T, V, dev), _rows(out, "out", torch.float32, T, V, dev)
+    T, V = x.shape
+    dev = x.get_device()
+    xs = _rows(x, "x", torch.float32, T, V, dev)
+    out, ys = (x, xs) if out is None else (out, _rows(out, "out", torch.float32, T, V, dev))
     if T > 1 and ys < V:
         raise ValueError("adjust: the rows of out must not overlap")
-    a = Rules()
+    n_tokens = n_bias = ts = bs = ms = 0
     if tokens is not None:
-        a.tokens_stride = _rows(tokens, "tokens", torch.int64, T, None, dev)
+        ts = _rows(tokens, "tokens", torch.int64, T, None, dev)
+        n_tokens = tokens.shape[1]
         _vector(length, "length", torch.int32, T, dev)
         if prompt is not None:
             _vector(prompt, "prompt", torch.int32, T, dev)
-        if (not torch.is_tensor(penalties) or penalties.dtype != torch.float32 or tuple(penalties.shape) != (T, 3)
-                or not penalties.is_contiguous() or penalties.device != dev):
+        if (not torch.is_tensor(penalties) or penalties.dtype != torch.float32 or penalties.shape != (T, 3)
+                or not penalties.is_contiguous() or penalties.get_device() != dev):
             raise ValueError(f"adjust: penalties must be contiguous float32 [{T}, 3] on the device of x")
-        if tokens.shape[1]:
-            a.tokens, a.length, a.prompt, a.penalties = _ptr(tokens), _ptr(length), _ptr(prompt), _ptr(penalties)
-            a.max_tokens = tokens.shape[1]
     elif length is not None or prompt is not None or penalties is not None:
         raise ValueError("adjust: length, prompt and penalties go with tokens")
     if bias_ids is not None or bias is not None:
-        a.bias_stride = _rows(bias_ids, "bias_ids", torch.int64, T, None, dev)
-        if _rows(bias, "bias", torch.float32, T, bias_ids.shape[1], dev) != a.bias_stride:
+        bs = _rows(bias_ids, "bias_ids", torch.int64, T, None, dev)
+        n_bias = bias_ids.shape[1]
+        if _rows(bias, "bias", torch.float32, T, n_bias, dev) != bs:
             raise ValueError("adjust: bias_ids and bias must have one layout")
-        if bias_ids.shape[1]:
-            a.bias_ids, a.bias, a.n_bias = _ptr(bias_ids), _ptr(bias), bias_ids.shape[1]
     if mask is not None:
-        a.mask_stride = _rows(mask, "mask", torch.int32, T, -(-V // 32), dev)
-        a.mask = _ptr(mask)
+        ms = _rows(mask, "mask", torch.int32, T, -(-V // 32), dev)
     if ids is not None:
         _vector(ids, "ids", torch.int64, T, dev)
     if T == 0:
         return out
+    if not n_tokens:
+        tokens = length = prompt = penalties = None
+    if not n_bias:
+        bias_ids = bias = None
+    a = Rules(_ptr(tokens), _ptr(length), _ptr(prompt), _ptr(penalties), _ptr(bias_ids), _ptr(bias), _ptr(mask), ts, bs,
+              ms, n_tokens, n_bias)
     L = lib()
-    with on(dev):
-        need = L.rv12_logits_workspace_bytes(V, T) if ids is not None else 0
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    device = x.device
+    with on(device):
+        need, ws = 0, None
+        if ids is not None:
+            need = L.rv12_logits_workspace_bytes(V, T)
+            ws = torch.empty(need, dtype=torch.uint8, device=device)
         check(L.rv12_logits_adjust(ctypes.byref(a), _ptr(x), xs, _ptr(out), ys, V, T, _ptr(ids), _ptr(ws), need,
-                                   _stream(dev)), "adjust")
+                                   _stream(device)), "adjust")
     return out

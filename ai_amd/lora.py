@@ -49,7 +49,8 @@ class Adapters:
             B = torch.cat([B, B.new_zeros(count, N, pad)], 2)
         self.A, self.B, self.scale = A.contiguous(), B.contiguous(), scale.contiguous()
         self.count, self.N, self.K, self.R, self.device = count, N, K, R, A.device
-        self._a = Lora(_ptr(self.A), _ptr(self.B), _ptr(self.scale), _ptr(self.ranks), N, K, self.A.shape[1], count)
+        self._index, self._r = A.get_device(), self.A.shape[1]
+        self._a = ctypes.byref(Lora(_ptr(self.A), _ptr(self.B), _ptr(self.scale), _ptr(self.ranks), N, K, self._r, count))
 
     @classmethod
     def from_pairs(cls, pairs, device="cuda"):
@@ -76,35 +77,40 @@ class Adapters:
         int32 [T], outside [0, count) (-1) no adapter: out[t] = y[t].  y and out:
         float32 [T, N], rows contiguous, any stride between them (a slice of a
         fused projection's output).  Can be captured in a HIP graph."""
-        dev, K, N = self.device, self.K, self.N
+        dev, K, N = self._index, self.K, self.N
         if mode not in (0, 1, 2):
             raise ValueError("apply: mode must be 0, 1 or 2")
-        if not torch.is_tensor(idx) or idx.dtype != torch.int32 or idx.dim() != 1 or not idx.is_contiguous() or idx.device != dev:
+        if (not torch.is_tensor(idx) or idx.dtype != torch.int32 or idx.dim() != 1 or not idx.is_contiguous()
+                or idx.get_device() != dev):
             raise ValueError("apply: idx must be a contiguous int32 vector on the adapters' device")
         T = idx.numel()
-        if (x.dtype != torch.float32 or not x.is_contiguous() or x.device != dev
-                or tuple(x.shape) != (T, 2 * K if mode == 2 else K)):
-            raise ValueError(f"apply: x must be contiguous float32 [{T}, {2 * K if mode == 2 else K}] on the adapters' device")
-        out = y if out is None else out
-        for t in (y, out):
-            if t.dtype != torch.float32 or tuple(t.shape) != (T, N) or t.device != dev or (N > 1 and t.stride(1) != 1):
-                raise ValueError(f"apply: y and out must be float32 [{T}, {N}], rows contiguous, on the adapters' device")
-            if T > 1 and t.stride(0) < N:
-                raise ValueError("apply: the rows of y and out must not overlap")
+        width = 2 * K if mode == 2 else K
+        if x.dtype != torch.float32 or x.shape != (T, width) or not x.is_contiguous() or x.get_device() != dev:
+            raise ValueError(f"apply: x must be contiguous float32 [{T}, {width}] on the adapters' device")
+        ys = self._stride(y, T)
+        out, os = (y, ys) if out is None else (out, self._stride(out, T))
         if lnw is not None:
             if mode == 2:
                 raise ValueError("apply: the RMSNorm goes with modes 0 and 1")
-            if lnw.dtype != torch.bfloat16 or tuple(lnw.shape) != (K,) or not lnw.is_contiguous() or lnw.device != dev:
+            if lnw.dtype != torch.bfloat16 or lnw.shape != (K,) or not lnw.is_contiguous() or lnw.get_device() != dev:
                 raise ValueError("apply: lnw must be a contiguous bf16 vector of K entries on the adapters' device")
         if T == 0:
             return out
         L = lib()
-        with on(dev):
-            need = L.rv12_lora_workspace_bytes(self._a.r, K, T)
+        with on(self.device):
+            need = L.rv12_lora_workspace_bytes(self._r, K, T)
             if need == 0:
                 raise ValueError("apply: at most 65536 rows")
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            check(L.rv12_lora_apply(ctypes.byref(self._a), _ptr(x), _ptr(y), y.stride(0) if T > 1 else N, _ptr(out),
-                                    out.stride(0) if T > 1 else N, _ptr(idx), T, _ptr(lnw), float(eps), int(mode),
-                                    _ptr(ws), need, _stream(dev)), "lora_apply")
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            check(L.rv12_lora_apply(self._a, _ptr(x), _ptr(y), ys, _ptr(out), os, _ptr(idx), T, _ptr(lnw), float(eps), mode,
+                                    _ptr(ws), need, _stream(self.device)), "lora_apply")
         return out
+
+    def _stride(self, t, T):
+        """Stride between the rows of y or out."""
+        if t.dtype != torch.float32 or t.shape != (T, self.N) or t.get_device() != self._index:
+            raise ValueError(f"apply: y and out must be float32 [{T}, {self.N}] on the adapters' device")
+        stride, one = t.stride()
+        if (one != 1 and self.N > 1) or (T > 1 and stride < self.N):
+            raise ValueError("apply: the rows of y and out must be contiguous and not overlap")
+        return stride if T > 1 else self.N
