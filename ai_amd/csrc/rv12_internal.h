@@ -204,7 +204,7 @@ inline int64_t paged_items(const PagedParams& p) {
 inline int paged_split_rows(const PagedParams& p) {
     return p.cap <= p.grain ? 0 : std::min(p.T, p.target / p.n_kv);
 }
-inline int paged_slots(const PagedParams& p) { return paged_split_rows(p) ? 2 * (p.target / p.n_kv) : 0; }
+inline int paged_slots(const PagedParams& p) { return paged_split_rows(p) ? 2 * p.target / p.n_kv : 0; }
 void launch_paged_append(const PagedParams& p, hipStream_t st);
 void launch_paged_attend(const PagedParams& p, hipStream_t st);
 

@@ -72,3 +72,48 @@ def test_object_refusals():
     with pytest.raises(ValueError):  # CPU tensors
         p.attend(z(1, 512), None, z(1, dtype=torch.int64), z(1, 1, dtype=torch.int32), z(1, 4, 16, 64), z(1, 4, 16, 64),
                  z(1, 512))
+
+
+def _plan(lens, n_kv, bf16, target=1024):
+    """The attention's plan as the kernel forms it: chunk length, chunks per row."""
+    total = sum((n + 31) // 32 for n in lens)
+    grain = 128 if bf16 else 64
+    up = lambda a, b: -(-a // b)
+    half = up(total * n_kv, target // 2) * 32
+    c = half if half <= 512 else max(up(total * n_kv, target) * 32, 512)
+    C = up(max(c, 1), grain) * grain
+    return C, [max(1, up(n, C)) for n in lens]
+
+
+@pytest.mark.parametrize("n_kv", [1, 2, 3, 5, 7, 8, 11, 16, 100, 256])
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_workspace_holds_every_plan(n_kv, bf16):
+    """Whatever the lengths, the partials of the rows in several chunks fit the
+    workspace, and the grid's workgroups cover every chunk (rows just past a
+    chunk's end need the most of both)."""
+    import random
+    from ai_amd import _lib
+    L = _lib.lib()
+    rng = random.Random(n_kv)
+    worst = 0
+    for _ in range(400):
+        T = rng.choice([1, 2, 3, 17, 64, 65, 200, 700])
+        pages = rng.choice([1, 9, 300, 4000])
+        cap = pages * 16
+        a = _paged(n_heads=n_kv, n_kv=n_kv, kv_bf16=bf16, max_pages=pages, table_stride=pages)
+        need = L.rv12_paged_attend_workspace_bytes(ctypes.byref(a), T)
+        assert need > 0
+        per_slot = n_kv * 16 * (128 + 4) * 4
+        room = (need - 16) // per_slot
+        base = rng.choice([0, rng.randint(1, cap), cap])
+        lens = [min(cap, max(0, rng.choice([base, base + 1, rng.randint(0, cap)]))) for _ in range(T)]
+        C, chunks = _plan(lens, n_kv, bf16)
+        # the rows' lengths just past multiples of that chunk length
+        for _ in range(3):
+            split = [c for c in chunks if c > 1]
+            assert sum(split) <= room and len(split) <= min(T, 1024 // n_kv)
+            assert sum(chunks) <= min(1024 // n_kv + T, T * -(-cap // (128 if bf16 else 64)))
+            worst = max(worst, sum(split) / max(room, 1))
+            lens = [min(cap, C * rng.randint(1, 2) + 1) for _ in range(T)]
+            C, chunks = _plan(lens, n_kv, bf16)
+    assert worst > 0.4  # the draws come near the bound
