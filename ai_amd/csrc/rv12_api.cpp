@@ -844,7 +844,7 @@ int rv12_paged_append(const rv12_paged* a, int t, const float* qkv, const float*
 size_t rv12_paged_attend_workspace_bytes(const rv12_paged* a, int t) {
     PagedParams p;
     if (paged_params(a, t, &p)) return 0;
-    return 16 + (size_t)paged_slots(p) * p.n_kv * (p.rt * p.g) * (p.head_dim + 4) * 4;
+    return 16 + paged_plan_bytes(p) + paged_part_bytes(p);
 }
 
 int rv12_paged_attend(const rv12_paged* a, int t, const float* q, const int32_t* seq, const int64_t* pos,
@@ -867,6 +867,10 @@ int rv12_paged_attend(const rv12_paged* a, int t, const float* q, const int32_t*
     p.vc = const_cast<void*>(vc);
     p.out = out;
     p.part = (float*)ws;
+    if (t > kPagedInlineRows) {
+        p.plan = (PlanItem*)((char*)ws + paged_part_bytes(p));
+        p.plan_items = (int)paged_items(p);
+    }
     launch_paged_attend(p, (hipStream_t)stream);
     return launch_status();
 }

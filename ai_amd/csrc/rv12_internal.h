@@ -172,6 +172,13 @@ constexpr int kMaxPrefillAttnTokens = 1 << 15;  // the prologue grid's second di
 int launch_prefill_attn(const AttnParams& p, hipStream_t st);
 
 // --- paged cache: append and attention of T token rows
+struct PlanItem {
+    int row, nr, n;     // leader row, rows, positions
+    int C;              // chunk length
+    int chunk, chunks;  // of this row
+    int slot;           // first partial of the row (rows of several chunks only)
+    int unused;
+};
 struct PagedParams {
     const float* qkv = nullptr;
     const float* qn = nullptr;
@@ -185,7 +192,9 @@ struct PagedParams {
     const float* q = nullptr;
     float* qo = nullptr;
     float* out = nullptr;
-    float* part = nullptr;  // [slots][n_kv][rt g][HD + 2] partials of rows in several chunks
+    float* part = nullptr;  // [slots][n_kv][rt g][HD + 4] partials of rows in several chunks
+    PlanItem* plan = nullptr;  // more than kPagedInlineRows rows: their plan
+    int plan_items = 0;        // entries of it before the rows of several chunks
     int T, n_heads, n_kv, head_dim, kv_bf16, page_log, n_seq;
     int g;   // query heads per kv head
     int rt;  // rows of one sequence that share a workgroup's 16 columns at most
@@ -195,6 +204,7 @@ struct PagedParams {
     float eps, scale;
 };
 constexpr int kMaxPagedRows = 1 << 16;
+constexpr int kPagedInlineRows = 64;
 // workgroups per kv head at most: every row has a chunk, and rows of n > C
 // positions have fewer than n / C + 1, the sum of n being at most C target / n_kv
 inline int64_t paged_items(const PagedParams& p) {
@@ -205,6 +215,12 @@ inline int paged_split_rows(const PagedParams& p) {
     return p.cap <= p.grain ? 0 : std::min(p.T, p.target / p.n_kv);
 }
 inline int paged_slots(const PagedParams& p) { return paged_split_rows(p) ? 2 * p.target / p.n_kv : 0; }
+inline size_t paged_part_bytes(const PagedParams& p) {
+    return (size_t)paged_slots(p) * p.n_kv * (p.rt * p.g) * (p.head_dim + 4) * 4;
+}
+inline size_t paged_plan_bytes(const PagedParams& p) {
+    return p.T <= kPagedInlineRows ? 0 : (size_t)(1 + paged_items(p) + paged_split_rows(p)) * sizeof(PlanItem);
+}
 void launch_paged_append(const PagedParams& p, hipStream_t st);
 void launch_paged_attend(const PagedParams& p, hipStream_t st);
 

@@ -228,59 +228,122 @@ __device__ __forceinline__ PlanRows plan_rows(const PagedParams& p, int base) {
     return o;
 }
 
-struct PlanItem {
-    int row, nr, n;     // leader row, rows, positions
-    int C;              // chunk length
-    int chunk, chunks;  // of this row
-    int slot;           // first partial of the row (rows of several chunks only)
-};
-
-// item `want` among the chunks of all rows, or (SEVERAL) row `want` among the rows
-// of several chunks.  False if there is none.  The chunk length: all positions
-// (in blocks of 32) over the target, in grains (one step of every wave).
-template <bool SEVERAL>
-__device__ __forceinline__ bool plan_find(const PagedParams& p, int want, PlanItem* it) {
-    const PlanRows r0 = plan_rows(p, 0);
-    int total = __builtin_amdgcn_readlane(wave_scan(r0.leader ? (r0.n + 31) >> 5 : 0), 63);
-    for (int base = 64; base < p.T; base += 64) {
-        const PlanRows o = plan_rows(p, base);
-        total += __builtin_amdgcn_readlane(wave_scan(o.leader ? (o.n + 31) >> 5 : 0), 63);
-    }
-    // up to 512 positions a chunk's own cost counts, and one workgroup per resident
-    // slot is best; above it smaller chunks even out the workgroups' ends
+// chunk length of the plan over `total` blocks of 32 positions
+__device__ __forceinline__ int plan_chunk(const PagedParams& p, int total) {
+    // up to 512 positions a chunk's own cost counts, and one workgroup per
+    // resident slot is best; above it smaller chunks even out the workgroups' ends
     // (1024 target: 8 rows of one sequence at 4096 positions, 64 query heads over 8,
     // 18.9 -> 16.9 us with half the workgroups; 64 rows of 500 to 8200 positions, 32
     // heads over 8, 142 us, 155 with half)
     const int64_t all = (int64_t)total * p.n_kv;
+    constexpr int64_t kKnee = 512;
     const int64_t half_c = (all + p.target / 2 - 1) / (p.target / 2) * 32;
-    const int64_t c = half_c <= 512 ? half_c : max((all + p.target - 1) / p.target * 32, (int64_t)512);
-    const int C = (int)((max(c, (int64_t)1) + p.grain - 1) & ~(int64_t)(p.grain - 1));
-    int items0 = 0, slots0 = 0;
-    for (int base = 0; base < p.T; base += 64) {
-        const PlanRows o = base ? plan_rows(p, base) : r0;
-        const int ch = o.leader ? max(1, (o.n + C - 1) / C) : 0;
-        const int sl = ch > 1 ? ch : 0;
-        const int mine = SEVERAL ? (ch > 1 ? 1 : 0) : ch;
-        // both sums at once: at most 2 target slots and target / n_kv + T items
-        const int both = wave_scan(sl << 18 | mine);
-        const int e = items0 + (both & 0x3FFFF) - mine;
-        const uint64_t hit = __ballot(want >= e && want < e + mine);
-        if (hit) {
-            const int s = __builtin_ctzll(hit);
-            it->row = base + s;
-            it->nr = __builtin_amdgcn_readlane(o.nr, s);
-            it->n = __builtin_amdgcn_readlane(o.n, s);
-            it->C = C;
-            it->chunk = want - __builtin_amdgcn_readlane(e, s);
-            it->chunks = __builtin_amdgcn_readlane(ch, s);
-            it->slot = slots0 + __builtin_amdgcn_readlane((both >> 18) - sl, s);
-            return true;
-        }
-        const int last = __builtin_amdgcn_readlane(both, 63);
-        items0 += last & 0x3FFFF;
-        slots0 += last >> 18;
+    const int64_t c = half_c <= kKnee ? half_c : max((all + p.target - 1) / p.target * 32, kKnee);
+    return (int)((max(c, (int64_t)1) + p.grain - 1) & ~(int64_t)(p.grain - 1));
+}
+__device__ __forceinline__ int plan_blocks(const PlanRows& o) { return o.leader ? (o.n + 31) >> 5 : 0; }
+__device__ __forceinline__ int plan_chunks(const PlanRows& o, int C) { return o.leader ? max(1, (o.n + C - 1) / C) : 0; }
+
+// item `want` among the chunks of all rows, or (SEVERAL) row `want` among the rows
+// of several chunks.  False if there is none.  Up to 64 rows every workgroup works
+// it out from one load of the rows; of more the list of k_paged_plan has it.
+template <bool SEVERAL>
+__device__ __forceinline__ bool plan_find(const PagedParams& p, int want, PlanItem* it) {
+    if (p.plan) {
+        if (want >= p.plan[0].row && !SEVERAL) return false;
+        if (want >= p.plan[0].nr && SEVERAL) return false;
+        *it = p.plan[1 + want + (SEVERAL ? p.plan_items : 0)];
+        return true;
     }
-    return false;
+    const PlanRows o = plan_rows(p, 0);
+    const int C = plan_chunk(p, __builtin_amdgcn_readlane(wave_scan(plan_blocks(o)), 63));
+    const int ch = plan_chunks(o, C), sl = ch > 1 ? ch : 0;
+    const int mine = SEVERAL ? (ch > 1 ? 1 : 0) : ch;
+    // both sums at once: at most 2 target slots and target + 64 items
+    const int both = wave_scan(sl << 16 | mine);
+    const int e = (both & 0xFFFF) - mine;
+    const uint64_t hit = __ballot(want >= e && want < e + mine);
+    if (!hit) return false;
+    const int s = __builtin_ctzll(hit);
+    it->row = s;
+    it->nr = __builtin_amdgcn_readlane(o.nr, s);
+    it->n = __builtin_amdgcn_readlane(o.n, s);
+    it->C = C;
+    it->chunk = want - __builtin_amdgcn_readlane(e, s);
+    it->chunks = __builtin_amdgcn_readlane(ch, s);
+    it->slot = __builtin_amdgcn_readlane((both >> 16) - sl, s);
+    return true;
+}
+
+// the plan of more than 64 rows, one workgroup: entry 0 the counts (row: items, nr:
+// rows of several chunks), then every item, then the rows of several chunks.  The
+// waves take the steps of 64 rows in turn, in three passes over them: the sum of
+// the positions, the numbers of items and slots, the entries.  (Worked out in every
+// workgroup, as for up to 64 rows, a prompt of 2048 rows took 850 us, not 206.)
+constexpr int kPlanThreads = 1024;
+__global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PagedParams p) {
+    constexpr int NW = kPlanThreads / 64;
+    __shared__ int sums[3][NW];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int steps = (p.T + 63) / 64;
+    const int s0 = (int)((int64_t)wv * steps / NW), s1 = (int)((int64_t)(wv + 1) * steps / NW);
+    int v = 0;
+    for (int s = s0; s < s1; ++s) v += plan_blocks(plan_rows(p, 64 * s));
+    v = wave_scan(v);
+    if (lane == 63) sums[0][wv] = v;
+    __syncthreads();
+    int total = 0;
+    for (int w = 0; w < NW; ++w) total += sums[0][w];
+    const int C = plan_chunk(p, total);
+    __syncthreads();
+    int items = 0, slots = 0, rows = 0;
+    for (int s = s0; s < s1; ++s) {
+        const int ch = plan_chunks(plan_rows(p, 64 * s), C);
+        items += ch;
+        slots += ch > 1 ? ch : 0;
+        rows += ch > 1 ? 1 : 0;
+    }
+    items = wave_scan(items);
+    slots = wave_scan(slots);
+    rows = wave_scan(rows);
+    if (lane == 63) {
+        sums[0][wv] = items;
+        sums[1][wv] = slots;
+        sums[2][wv] = rows;
+    }
+    __syncthreads();
+    items = slots = rows = 0;
+    for (int w = 0; w < wv; ++w) {
+        items += sums[0][w];
+        slots += sums[1][w];
+        rows += sums[2][w];
+    }
+    if (threadIdx.x == kPlanThreads - 1) {
+        p.plan[0].row = items + sums[0][NW - 1];
+        p.plan[0].nr = rows + sums[2][NW - 1];
+    }
+    for (int s = s0; s < s1; ++s) {
+        const PlanRows o = plan_rows(p, 64 * s);
+        const int ch = plan_chunks(o, C), sl = ch > 1 ? ch : 0, se = ch > 1 ? 1 : 0;
+        const int ie = wave_scan(ch), le = wave_scan(sl), re = wave_scan(se);
+        PlanItem it;
+        it.row = 64 * s + lane;
+        it.nr = o.nr;
+        it.n = o.n;
+        it.C = C;
+        it.chunks = ch;
+        it.slot = slots + le - sl;
+        it.chunk = 0;
+        it.unused = 0;
+        if (se) p.plan[1 + p.plan_items + rows + re - 1] = it;
+        for (int i = 0; i < ch; ++i) {
+            it.chunk = i;
+            p.plan[1 + items + ie - ch + i] = it;
+        }
+        items += __builtin_amdgcn_readlane(ie, 63);
+        slots += __builtin_amdgcn_readlane(le, 63);
+        rows += __builtin_amdgcn_readlane(re, 63);
+    }
 }
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -720,6 +783,7 @@ static void launch_paged_t(const PagedParams& p, hipStream_t st) {
 }
 
 void launch_paged_attend(const PagedParams& p, hipStream_t st) {
+    if (p.plan) hipLaunchKernelGGL(k_paged_plan, dim3(1), dim3(kPlanThreads), 0, st, p);
     if (p.head_dim == 128) {
         if (p.kv_bf16) launch_paged_t<128, true>(p, st);
         else launch_paged_t<128, false>(p, st);

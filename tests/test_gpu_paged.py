@@ -402,3 +402,56 @@ def test_refusals():
         with pytest.raises(ValueError):
             p.append(**{**a, **bad})
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("H,KV,HD", HEADS)
+@pytest.mark.parametrize("kv", KV_TYPES)
+def test_attend_prompts(H, KV, HD, kv):
+    """Whole prompts and long chunks (the plan of more than 64 rows): runs that end
+    inside a wave's rows, rows out of order and padding among them, NaN past a run's
+    end and in its last position."""
+    from ai_amd.attn import PagedRopeAttn
+    page = 16
+    g = _gen(H, KV, HD, 9)
+    lens = [333, 70]
+    print("case", H, KV, HD, kv, flush=True)
+    table, n_pages = _table(lens, page, g)
+    kc, vc = _randn(g, n_pages, KV, page, HD).to(kv), _randn(g, n_pages, KV, page, HD).to(kv)
+    end = int(table[0, 332 // page])
+    kc[end, :, 332 % page + 1:], vc[end, :, 332 % page + 1:] = float("nan"), float("inf")
+    rows = [(0, j) for j in range(333)] + [(1, j) for j in range(70)] + [(-1, 0)] * 3 + \
+        [(0, j) for j in range(290, 233, -1)] + [(1, 5), (0, 6), (1, 7)]
+    seq = torch.tensor([r[0] for r in rows], dtype=torch.int32, device="cuda")
+    pos = torch.tensor([r[1] for r in rows], device="cuda")
+    q = _randn(g, len(rows), H * HD) * 2
+    p = PagedRopeAttn(H, KV, HD, page, kv, EPS)
+    out = _check(p, q, seq, pos, table, kc, vc)
+    # one sequence from the middle, rows at an odd start
+    _check(p, q[101:333].contiguous(), seq[101:333].contiguous(), pos[101:333].contiguous(), table[:1], kc, vc)
+    # its last position NaN: the rows of that position alone have it
+    kc[end, :, 332 % page], vc[end, :, 332 % page] = float("nan"), float("inf")
+    o2 = torch.empty_like(out)
+    p.attend(q, seq, pos, table, kc, vc, o2)
+    hit = (seq == 0) & (pos == 332)
+    assert bool(o2[hit].isnan().all()) and torch.equal(o2[~hit], out[~hit])
+
+
+@pytest.mark.parametrize("kv", KV_TYPES)
+def test_attend_prompt_behind_a_long_context(kv):
+    """40 rows behind 9000 positions (their chunks joined), missing pages among them."""
+    from ai_amd.attn import PagedRopeAttn
+    for H, KV in ((32, 8), (64, 8), (16, 1)):
+        page, HD, n = 64, 128, 9040
+        g = _gen(H, 10)
+        table, n_pages = _table([n], page, g)
+        table[0, 20:40] = -1
+        kc, vc = _randn(g, n_pages, KV, page, HD).to(kv), _randn(g, n_pages, KV, page, HD).to(kv)
+        pos = torch.arange(n - 40, n, device="cuda")
+        q = _randn(g, 40, H * HD)
+        p = PagedRopeAttn(H, KV, HD, page, kv, EPS)
+        print("case", H, KV, kv, flush=True)
+        seq = torch.zeros(40, dtype=torch.int32, device="cuda")
+        a = _check(p, q, seq, pos, table, kc, vc)
+        b = torch.empty_like(a)
+        p.attend(q, seq, pos, table, kc, vc, b)
+        assert torch.equal(a, b)

@@ -74,10 +74,9 @@ def test_object_refusals():
                  z(1, 512))
 
 
-def _plan(lens, n_kv, bf16, target=1024):
+def _plan(lens, n_kv, grain, target=1024):
     """The attention's plan as the kernel forms it: chunk length, chunks per row."""
     total = sum((n + 31) // 32 for n in lens)
-    grain = 128 if bf16 else 64
     up = lambda a, b: -(-a // b)
     half = up(total * n_kv, target // 2) * 32
     c = half if half <= 512 else max(up(total * n_kv, target) * 32, 512)
@@ -95,7 +94,7 @@ def test_workspace_holds_every_plan(n_kv, bf16):
     from ai_amd import _lib
     L = _lib.lib()
     rng = random.Random(n_kv)
-    worst = 0
+    worst, grain = 0, 128 if bf16 else 64
     for _ in range(400):
         T = rng.choice([1, 2, 3, 17, 64, 65, 200, 700])
         pages = rng.choice([1, 9, 300, 4000])
@@ -104,16 +103,18 @@ def test_workspace_holds_every_plan(n_kv, bf16):
         need = L.rv12_paged_attend_workspace_bytes(ctypes.byref(a), T)
         assert need > 0
         per_slot = n_kv * 16 * (128 + 4) * 4
-        room = (need - 16) // per_slot
+        items, rows = min(1024 // n_kv + T, T * -(-cap // grain)), min(T, 1024 // n_kv) if cap > grain else 0
+        room, rest = divmod(need - 16 - (32 * (1 + items + rows) if T > 64 else 0), per_slot)
+        assert rest == 0
         base = rng.choice([0, rng.randint(1, cap), cap])
         lens = [min(cap, max(0, rng.choice([base, base + 1, rng.randint(0, cap)]))) for _ in range(T)]
-        C, chunks = _plan(lens, n_kv, bf16)
+        C, chunks = _plan(lens, n_kv, grain)
         # the rows' lengths just past multiples of that chunk length
         for _ in range(3):
             split = [c for c in chunks if c > 1]
-            assert sum(split) <= room and len(split) <= min(T, 1024 // n_kv)
-            assert sum(chunks) <= min(1024 // n_kv + T, T * -(-cap // (128 if bf16 else 64)))
+            assert sum(split) <= room and len(split) <= rows
+            assert sum(chunks) <= items
             worst = max(worst, sum(split) / max(room, 1))
             lens = [min(cap, C * rng.randint(1, 2) + 1) for _ in range(T)]
-            C, chunks = _plan(lens, n_kv, bf16)
+            C, chunks = _plan(lens, n_kv, grain)
     assert worst > 0.4  # the draws come near the bound
