@@ -381,7 +381,7 @@ const char* rv12_strerror(int s) {
         case RV12_E_SCRATCH: return "workspace of the launch exceeds the static scratch (RV12_STATIC_SCRATCH_BYTES, 8 MiB)";
         case RV12_E_PAGED:
             return "bad paged cache or rows (head_dim 64 or 128, up to 16 query heads per kv head, pages of 16 .. 1024 "
-                   "positions in powers of two, T in [1, 65536], table positions below 2^31 - 4096)";
+                   "positions in powers of two, T in [1, 65536], at most 2^30 positions in a table row)";
         case RV12_E_RULES: return "bad logits or rules (T in [1, 65535], V in [1, 2^31 - 65536), counts and strides >= 0)";
         case RV12_E_LORA:
             return "bad adapters (N >= 1, K % 32 == 0, rank a multiple of 8 up to 128, count >= 1) or T outside [1, 65536]";
@@ -795,7 +795,8 @@ static int paged_params(const rv12_paged* a, int t, PagedParams* p) {
     if (a->n_seq < 1 || a->max_pages < 1 || a->n_pages < 1 || a->n_pages > 0x7FFFFFFF || a->table_stride < a->max_pages)
         return RV12_E_PAGED;
     const int64_t cap = (int64_t)a->max_pages * a->page;
-    if (cap > (int64_t)0x7FFFFFFF - 4096 || t < 1 || t > kMaxPagedRows) return RV12_E_PAGED;
+    // (a position plus a chunk length stays an int)
+    if (cap > (int64_t)1 << 30 || t < 1 || t > kMaxPagedRows) return RV12_E_PAGED;
     p->T = t;
     p->n_heads = a->n_heads;
     p->n_kv = a->n_kv;

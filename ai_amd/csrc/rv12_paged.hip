@@ -126,7 +126,7 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedParams p) {
 }
 
 void launch_paged_append(const PagedParams& p, hipStream_t st) {
-    // every head of a row at once while the rows are few
+    // every head of a row at once
     const int slots = 256 / (p.head_dim / 8), nh = p.n_heads + 2 * p.n_kv;
     const dim3 grid((unsigned)p.T, (unsigned)((nh + slots - 1) / slots));
     if (p.head_dim == 128) {

@@ -361,8 +361,8 @@ int rv12_prefill_rope_attn(const rv12_attn* a, int t, const float* qkv, const fl
  * graph can advance them.  A row whose sequence is outside [0, n_seq) or whose
  * position is outside [0, max_pages page) is padding.  A page id outside
  * [0, n_pages) is no page.  head_dim 64 or 128; n_heads / n_kv 1 .. 16; page a
- * power of two, 16 .. 1024; max_pages page below 2^31 - 4096, t max_pages page at
- * most 2^35 and times n_kv 2^40. */
+ * power of two, 16 .. 1024; max_pages page at most 2^30, t max_pages page at most
+ * 2^35 and times n_kv 2^40. */
 typedef struct rv12_paged {
     int32_t n_heads, n_kv, head_dim, page;
     int32_t kv_bf16; /* 1: bf16 caches, 0: float32 */
@@ -391,9 +391,11 @@ int rv12_paged_append(const rv12_paged* a, int t, const float* qkv, const float*
  * positions, the rows' own among them, are in the cache before the call.
  * Positions without a page take no part; a row that is padding, or has nothing
  * left to attend, gives zeros.  Slots past a row's position are not read into it,
- * whatever they hold.  Two passes (chunks of positions, about 1024 workgroups
- * whatever the lengths; the join of the rows in several chunks, in chunk order),
- * no atomics.  ws: rv12_paged_attend_workspace_bytes(a, t) bytes, 16-byte aligned
+ * whatever they hold; an infinite key or value that it sees gives NaN.  The chunks of
+ * positions, about 1024 workgroups whatever the lengths, and so a result's last bits
+ * depend on the lengths of all rows.  Two passes (the chunks; the join of the rows
+ * in several, in chunk order), before them for more than 64 rows a small one that
+ * lists the chunks; no atomics.  ws: rv12_paged_attend_workspace_bytes(a, t) bytes, 16-byte aligned
  * (0 bytes there: a or t out of range); calls that overlap need their own.  The
  * paged counterpart of rope_attn_k's and attn_k's attention,
  * ramvi/engine/ramvi_engine/kernels/tkernels.py:123-213. */

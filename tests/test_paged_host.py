@@ -15,7 +15,8 @@ def _paged(**kw):
 
 
 BAD = [dict(head_dim=96), dict(n_heads=31), dict(n_kv=0), dict(n_heads=136), dict(page=8), dict(page=48), dict(page=2048),
-       dict(n_seq=0), dict(max_pages=0), dict(n_pages=0), dict(table_stride=7), dict(max_pages=1 << 27, table_stride=1 << 27)]
+       dict(n_seq=0), dict(max_pages=0), dict(n_pages=0), dict(table_stride=7), dict(max_pages=1 << 27, table_stride=1 << 27),
+       dict(max_pages=(1 << 26) + 1, table_stride=1 << 27)]
 
 
 @pytest.mark.parametrize("kw", BAD)
