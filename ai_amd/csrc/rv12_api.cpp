@@ -968,8 +968,7 @@ int rv12_lora_apply(const rv12_lora* a, const float* x, const float* y, int64_t 
     p.eps = eps;
     p.h = (float*)ws;
     p.ssq = p.h + (size_t)p.S * t * 16 * lora_rank_blocks(a->r);
-    const bool vec = aligned16(y) && aligned16(out) && a->n % 4 == 0 && (t == 1 || (y_stride % 4 == 0 && out_stride % 4 == 0));
-    launch_lora(p, vec, (hipStream_t)stream);
+    launch_lora(p, (hipStream_t)stream);
     return launch_status();
 }
 

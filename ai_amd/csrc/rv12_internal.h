@@ -288,7 +288,7 @@ inline void lora_launch(LoraParams* p) {
     p->nbw = 16;
     while (p->nbw > 1 && (int64_t)((nblk + 4 * p->nbw - 1) / (4 * p->nbw)) * tiles * p->slots < 256) p->nbw /= 2;
 }
-void launch_lora(const LoraParams& p, bool vec, hipStream_t st);
+void launch_lora(const LoraParams& p, hipStream_t st);
 
 int launch_gemv(const LinearParams& p, int T, int rb, int waves, int splits, hipStream_t st);
 // ks: the waves of a workgroup split its K steps (kernel 3) instead of its rows (kernel 2)

@@ -146,15 +146,22 @@ __global__ __launch_bounds__(256) void k_lora_down(LoraParams p) {
 // the RMSNorm's.  The workgroup adds the splits' h (every thread one part of it, all
 // loads at once) and leaves it in LDS as the products' operand; then a wave takes
 // p.nbw consecutive blocks of 16 output rows, UB at a time, the weights and y of
-// the next UB loaded ahead of the products and stores of these.
-template <int RB, bool VEC>  // VEC: y and out rows at 16-byte addresses, N % 4 == 0
-__global__ __launch_bounds__(256) void k_lora_up(LoraParams p) {
+// the next UB loaded ahead of the products and stores of these.  The products leave
+// 4 rows of a token per lane; they go through LDS to whole token rows, so that y is
+// read and out written in runs of 64 UB bytes.
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // at any float's address
+
+template <int RB>
+__global__ __launch_bounds__(256, RB == 8 ? 2 : 3) void k_lora_up(LoraParams p) {
     constexpr int RS = (RB + 1) / 2;  // steps of 32 ranks
     constexpr int UB = RB == 8 ? 2 : 4;
+    constexpr int LR = 4 * UB, RI = 64 / LR;  // lanes of one token row, rows at once (UB times)
+    constexpr int kRow = 16 * UB + 4;         // LDS floats of a token row
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q4 = lane >> 4, c16 = lane & 15;
-    const int t0 = blockIdx.y * 16, t = t0 + c16;
+    const int tr = lane / LR, cr = 4 * (lane % LR);  // the lane's first token row and its 4 outputs
+    const int t0 = blockIdx.y * 16;
     const int nb0 = (blockIdx.x * 4 + wv) * p.nbw, nb1 = min(nb0 + p.nbw, (p.N + 15) / 16);
     constexpr int HE = 64 * RB;             // float4 parts of the tile's h
     constexpr int GR = HE < 256 ? 256 / HE : 1;  // thread groups that share the splits
@@ -162,33 +169,40 @@ __global__ __launch_bounds__(256) void k_lora_up(LoraParams p) {
     __shared__ f32x4 part[GR][HE];
     __shared__ u32x4 hl[RS][3][64];
     __shared__ float factor[16];
+    __shared__ __align__(16) float sums[4][16 * kRow];
     for (int slot = blockIdx.z;; slot += gridDim.z) {
         int id;
         bool mine;
         if (!tile_slot(p, t0, slot, &id, &mine)) return;
         if (id < 0 && p.y == p.out) continue;
+        const uint32_t rows = (uint32_t)__ballot(mine);  // bit of every token row
         const int rank = id < 0 ? 0 : (p.ranks ? min(max(p.ranks[id], 0), p.R) : p.R);
         const uint16_t* B = p.B + (int64_t)max(id, 0) * p.N * p.R + 8 * q4;
         u32x4 bv[UB][RS];
         f32x4 yv[UB];
         auto load = [&](int nb) {
+            const int n1 = min(16 * nb1, p.N);
 #pragma unroll
             for (int u = 0; u < UB; ++u) {
-                if (nb + u >= nb1) break;
-                const int n = min(16 * (nb + u) + c16, p.N - 1), no = 16 * (nb + u) + 4 * q4;
+                const int n = min(16 * (nb + u) + c16, p.N - 1);
 #pragma unroll
                 for (int s = 0; s < RS; ++s) {
                     bv[u][s] = u32x4{0, 0, 0, 0};
-                    if (32 * s < rank && 32 * s + 8 * q4 < p.R)
+                    if (nb + u < nb1 && 32 * s < rank && 32 * s + 8 * q4 < p.R)
                         bv[u][s] = *reinterpret_cast<const u32x4*>(B + (int64_t)n * p.R + 32 * s);
                 }
-                const float* y = p.y + (int64_t)t * p.y_stride + no;
-                if constexpr (VEC) {
-                    if (mine && no < p.N) yv[u] = *reinterpret_cast<const f32x4*>(y);
-                } else {
+            }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (mine && no + e < p.N) yv[u][e] = y[e];
+            for (int u = 0; u < UB; ++u) {
+                const int t = u * RI + tr, no = 16 * nb + cr;
+                const float* y = p.y + (int64_t)(t0 + t) * p.y_stride + no;
+                if (rows >> t & 1u) {
+                    if (no + 4 <= n1) {
+                        yv[u] = *reinterpret_cast<const f32x4u*>(y);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) yv[u][e] = no + e < n1 ? y[e] : 0.0f;
+                    }
                 }
             }
         };
@@ -246,53 +260,63 @@ __global__ __launch_bounds__(256) void k_lora_up(LoraParams p) {
                 for (int c = 0; c < 3; ++c) hp[s][c] = hl[s][c][lane];
         }
         for (int nb = nb0; nb < nb1; nb += UB) {
-            f32x4 acc[UB];
+            const int n1 = min(16 * nb1, p.N);
+            float* tile = sums[wv];
 #pragma unroll
             for (int u = 0; u < UB; ++u) {
-                acc[u] = f32x4{0, 0, 0, 0};
+                f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
                 for (int s = 0; s < RS; ++s) {
                     if (32 * s >= rank) break;
 #pragma unroll
-                    for (int c = 0; c < 3; ++c) acc[u] = mfma(bv[u][s], hp[s][c], acc[u]);
+                    for (int c = 0; c < 3; ++c) acc = mfma(bv[u][s], hp[s][c], acc);
                 }
-                acc[u] += yv[u];
+                *reinterpret_cast<f32x4*>(tile + c16 * kRow + 16 * u + 4 * q4) = acc;
             }
+            f32x4 yo[UB];
+#pragma unroll
+            for (int u = 0; u < UB; ++u) yo[u] = yv[u];
             if (nb + UB < nb1) load(nb + UB);
+            // (a wave's LDS accesses keep their order: its own rows are there)
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int u = 0; u < UB; ++u) {
-                const int no = 16 * (nb + u) + 4 * q4;
-                if (!mine || nb + u >= nb1) continue;
-                float* o = p.out + (int64_t)t * p.out_stride + no;
-                if constexpr (VEC) {
-                    if (no < p.N) *reinterpret_cast<f32x4*>(o) = acc[u];
-                } else {
+                const int t = u * RI + tr, no = 16 * nb + cr;
+                const f32x4 o = yo[u] + *reinterpret_cast<const f32x4*>(tile + t * kRow + cr);
+                float* out = p.out + (int64_t)(t0 + t) * p.out_stride + no;
+                if (rows >> t & 1u) {
+                    if (no + 4 <= n1) {
+                        *reinterpret_cast<f32x4u*>(out) = o;
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (no + e < p.N) o[e] = acc[u][e];
+                        for (int e = 0; e < 4; ++e)
+                            if (no + e < n1) out[e] = o[e];
+                    }
                 }
             }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
     }
 }
 
 template <int RB>
-static void launch_lora_t(const LoraParams& p, bool vec, hipStream_t st) {
+static void launch_lora_t(const LoraParams& p, hipStream_t st) {
     const unsigned tiles = (unsigned)((p.T + 15) / 16), nblk = (unsigned)((p.N + 15) / 16);
     const dim3 d((unsigned)p.S, tiles, (unsigned)p.slots);
     if (p.mode == 2) hipLaunchKernelGGL((k_lora_down<RB, true>), d, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((k_lora_down<RB, false>), d, dim3(256), 0, st, p);
     const dim3 g((nblk + 4 * p.nbw - 1) / (4 * p.nbw), tiles, (unsigned)p.slots);
-    if (vec) hipLaunchKernelGGL((k_lora_up<RB, true>), g, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((k_lora_up<RB, false>), g, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((k_lora_up<RB>), g, dim3(256), 0, st, p);
 }
 
-void launch_lora(const LoraParams& p, bool vec, hipStream_t st) {
+void launch_lora(const LoraParams& p, hipStream_t st) {
     switch (lora_rank_blocks(p.R)) {
-        case 1: launch_lora_t<1>(p, vec, st); break;
-        case 2: launch_lora_t<2>(p, vec, st); break;
-        case 4: launch_lora_t<4>(p, vec, st); break;
-        default: launch_lora_t<8>(p, vec, st); break;
+        case 1: launch_lora_t<1>(p, st); break;
+        case 2: launch_lora_t<2>(p, st); break;
+        case 4: launch_lora_t<4>(p, st); break;
+        default: launch_lora_t<8>(p, st); break;
     }
 }
 
