@@ -382,7 +382,9 @@ const char* rv12_strerror(int s) {
         case RV12_E_PAGED:
             return "bad paged cache or rows (head_dim 64 or 128, up to 16 query heads per kv head, pages of 16 .. 1024 "
                    "positions in powers of two, T in [1, 65536], at most 2^30 positions in a table row)";
-        case RV12_E_RULES: return "bad logits or rules (T in [1, 65535], V in [1, 2^31 - 65536), counts and strides >= 0)";
+        case RV12_E_RULES: return 
+            "bad logits or rules (T in [1, 65535], V in [1, 2^31 - 65536), fewer than 2^20 tokens and 2048 biases a row, "
+            "strides >= 0)";
         case RV12_E_LORA:
             return "bad adapters (N >= 1, K % 32 == 0, rank a multiple of 8 up to 128, count >= 1) or T outside [1, 65536]";
         case RV12_E_LAUNCH: return "kernel launch failed";
@@ -887,7 +889,7 @@ int rv12_logits_adjust(const rv12_rules* rules, const float* x, int64_t x_stride
     if (!rules || !x || !y) return RV12_E_NULL;
     const rv12_rules& a = *rules;
     if (!rv12_logits_workspace_bytes(v, t)) return RV12_E_RULES;
-    if (a.max_tokens < 0 || a.n_bias < 0 || a.tokens_stride < 0 || a.bias_stride < 0 || a.mask_stride < 0 ||
+    if (a.max_tokens < 0 || a.max_tokens >= 1 << kAdjustCountBits || a.n_bias < 0 || a.n_bias > 2047 || a.tokens_stride < 0 || a.bias_stride < 0 || a.mask_stride < 0 ||
         x_stride < 0 || (t > 1 && y_stride < v))
         return RV12_E_RULES;
     if (a.tokens && (!a.length || !a.penalties)) return RV12_E_NULL;

@@ -226,6 +226,7 @@ void launch_paged_attend(const PagedParams& p, hipStream_t st);
 
 // --- rules on logits (k_adjust)
 constexpr int kAdjustThreads = 256;
+constexpr int kAdjustCountBits = 20;  // a token counts up to 2^20 - 1 times; the 11 bits above hold 2047 bias entries
 struct AdjustParams {
     const float* x;
     float* y;

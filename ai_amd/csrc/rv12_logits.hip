@@ -19,9 +19,9 @@
 
 namespace rv12 {
 
-// counts of a slice: bit 31 set once the id is among the row's tokens, bit 30 once
-// it has a bias, below them the generated tokens
-constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u;
+// the word of an id: bit 31 set once it is among the row's tokens, bits 20 .. 30 the
+// place of its last bias entry plus one, below them how often it was generated
+constexpr uint32_t kSeen = 0x80000000u, kCount = (1u << kAdjustCountBits) - 1u;
 constexpr int kNoId = 0x7FFFFFFF;
 
 // four floats at a 4-byte address (one 16-byte access all the same): rows of an odd
@@ -32,9 +32,8 @@ __global__ __launch_bounds__(kAdjustThreads) void k_adjust(AdjustParams p) {
     constexpr int U = 4;               // 16-byte loads of a thread in flight
     constexpr int TB = 8;              // tokens of a thread in flight
     constexpr int kStep = 4 * kAdjustThreads;
-    extern __shared__ u32x4 lds[];     // counts [slice], then the bias entries' places [slice]
-    uint32_t* cnt = reinterpret_cast<uint32_t*>(lds);
-    int* bias_at = reinterpret_cast<int*>(cnt + p.slice);
+    extern __shared__ u32x4 lds[];     // the slice's words
+    uint32_t* word = reinterpret_cast<uint32_t*>(lds);
     const int r = blockIdx.y, t = threadIdx.x, lane = t & 63;
     const int64_t n0 = (int64_t)blockIdx.x * p.slice;
     const int ns = (int)min((int64_t)p.slice, p.V - n0);
@@ -71,33 +70,30 @@ __global__ __launch_bounds__(kAdjustThreads) void k_adjust(AdjustParams p) {
 #pragma unroll
         for (int u = 0; u < TB; ++u) n[u] = L ? tok[min(t + u * kAdjustThreads, L - 1)] : 0;
         int64_t nb = t < p.n_bias ? id[t] : -1;
-        for (int i = t; i < p.slice / 4; i += kAdjustThreads) {
-            lds[i] = u32x4{0, 0, 0, 0};
-            if (p.n_bias) lds[p.slice / 4 + i] = u32x4{0, 0, 0, 0};
-        }
+        for (int i = t; i < p.slice / 4; i += kAdjustThreads) lds[i] = u32x4{0, 0, 0, 0};
         __syncthreads();
+        if (p.n_bias) {  // the biases first, while a word holds nothing else: the last entry of an id stays
+            for (int i = t; i < p.n_bias; i += kAdjustThreads) {
+                const int64_t k = nb - n0;
+                if (k >= 0 && k < ns) atomicMax(&word[k], (uint32_t)(i + 1) << kAdjustCountBits);
+                if (i + kAdjustThreads < p.n_bias) nb = id[i + kAdjustThreads];
+            }
+            __syncthreads();
+        }
         for (int i0 = t; i0 < L; i0 += TB * kAdjustThreads) {
 #pragma unroll
             for (int u = 0; u < TB; ++u) {
                 const int i = i0 + u * kAdjustThreads;
                 const int64_t k = n[u] - n0;
                 if (i < L && k >= 0 && k < ns) {
-                    atomicOr(&cnt[k], kSeen);
-                    if (i >= made) atomicAdd(&cnt[k], 1u);
+                    atomicOr(&word[k], kSeen);
+                    if (i >= made) atomicAdd(&word[k], 1u);
                 }
             }
             if (i0 + TB * kAdjustThreads < L) {
 #pragma unroll
                 for (int u = 0; u < TB; ++u) n[u] = tok[min(i0 + (TB + u) * kAdjustThreads, L - 1)];
             }
-        }
-        for (int i = t; i < p.n_bias; i += kAdjustThreads) {
-            const int64_t k = nb - n0;
-            if (k >= 0 && k < ns) {
-                atomicOr(&cnt[k], kBiased);
-                atomicMax(&bias_at[k], i);  // the last entry of an id counts
-            }
-            if (i + kAdjustThreads < p.n_bias) nb = id[i + kAdjustThreads];
         }
         __syncthreads();
     }
@@ -123,10 +119,11 @@ __global__ __launch_bounds__(kAdjustThreads) void k_adjust(AdjustParams p) {
                     float f = v[u][e];
                     if (c[e] & kSeen) {
                         f = f > 0.0f ? f / rep : f * rep;
-                        const uint32_t k = c[e] & ~(kSeen | kBiased);
+                        const uint32_t k = c[e] & kCount;
                         if (k) f -= freq * (float)k + pres;
                     }
-                    if (c[e] & kBiased) f += bias[bias_at[i + e]];
+                    const uint32_t b = (c[e] & ~kSeen) >> kAdjustCountBits;
+                    if (b) f += bias[b - 1];
                     v[u][e] = f;
                 }
             }
@@ -207,7 +204,7 @@ void launch_adjust(const AdjustParams& pa, int T, int64_t* ids, hipStream_t st) 
     AdjustParams p = pa;
     const int ns = (int)((p.V + p.slice - 1) / p.slice);
     hipLaunchKernelGGL(k_adjust, dim3((unsigned)ns, (unsigned)T), dim3(kAdjustThreads),
-                       (size_t)p.slice * (p.n_bias ? 8 : 4), st, p);
+                       (size_t)p.slice * 4, st, p);
     if (ids) hipLaunchKernelGGL(k_adjust_pick, dim3((unsigned)T), dim3(64), 0, st, p.pv, p.pi, ns, ids);
 }
 

@@ -48,7 +48,7 @@ def adjust(x, out=None, tokens=None, length=None, prompt=None, penalties=None, b
                smallest on ties, NaN counting as the largest, -1 where the mask
                allows none
 
-    Ids outside [0, V), such as the -1 of an unused entry, are passed over.  All on
+    L is below 2^20 and M below 2^11.  Ids outside [0, V), such as the -1 of an unused entry, are passed over.  All on
     one GPU; nothing is read back, so a call can be captured in a HIP graph."""
     if not torch.is_tensor(x) or not x.is_cuda:
         raise ValueError("adjust: x must be a tensor on the GPU")

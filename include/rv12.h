@@ -415,7 +415,7 @@ int rv12_paged_attend(const rv12_paged* a, int t, const float* q, const int32_t*
  * repetition, frequency, presence (NULL with tokens NULL); bias_ids / bias: n_bias
  * entries per row; mask: bit n & 31 of word n >> 5 of the row set where id n is
  * allowed.  Ids outside [0, v) in tokens and bias_ids are passed over.  Every
- * part may be absent (NULL).  Strides are in elements, from row to row.  A field's
+ * part may be absent (NULL).  max_tokens below 2^20, n_bias below 2^11.  Strides are in elements, from row to row.  A field's
  * rows may all be one (stride 0). */
 typedef struct rv12_rules {
     const int64_t* tokens;

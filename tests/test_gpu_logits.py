@@ -162,6 +162,25 @@ def test_histories_longer_than_the_rows_tokens():
     assert ids == _pick(y, ok)
 
 
+def test_the_largest_counts():
+    """2047 biases of one row and a token seen 2^20 - 1 times, generated all or all
+    but some; the counts beside the biases of the same ids."""
+    V, L, M = 5000, (1 << 20) - 1, 2047
+    rng = np.random.default_rng(9)
+    x = rng.standard_normal((2, V)).astype(np.float32)
+    tok = np.full((2, L), 17)
+    tok[1, ::3] = 18
+    bias_ids = np.stack([rng.permutation(V)[:M], np.full(M, 17)])
+    bias_ids[0, 5] = 17
+    a = {"tokens": tok, "length": np.full(2, L, np.int32), "prompt": np.array([0, 1000], np.int32),
+         "penalties": np.float32([[1.2, 1e-5, 0.5], [1.2, 1e-5, 0.5]]), "bias_ids": bias_ids,
+         "bias": rng.standard_normal((2, M)).astype(np.float32)}
+    y, ids, _ = _run(x, a)
+    ref, bound, ok = _ref(x, **a)
+    _same(y, ref, bound)
+    assert ids == _pick(y, ok)
+
+
 def test_strides_expanded_rows_and_streams():
     """Rows of wider tensors, one history and mask for all rows (stride 0), odd row
     addresses, a side stream, and a captured call replayed with other inputs."""

@@ -25,6 +25,8 @@ def test_rules_abi():
         r = _lib.Rules()
         setattr(r, f, -1)
         assert call(r) == _lib.RV12_E_RULES, f
+    for kw in (dict(max_tokens=1 << 20), dict(n_bias=2048)):
+        assert call(_lib.Rules(**kw)) == _lib.RV12_E_RULES
     r = _lib.Rules(tokens=P, max_tokens=4)
     assert call(r) == _lib.RV12_E_NULL  # no length, no penalties
     r = _lib.Rules(n_bias=4, bias_ids=P)
