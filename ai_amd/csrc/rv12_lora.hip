@@ -207,7 +207,6 @@ __global__ __launch_bounds__(256, RB == 8 ? 2 : 3) void k_lora_up(LoraParams p) 
             }
         };
         load(nb0);
-        u32x4 hp[RS][3];
         if (rank > 0) {  // (the same for the whole workgroup)
             const int tid = threadIdx.x;
             {
@@ -254,14 +253,18 @@ __global__ __launch_bounds__(256, RB == 8 ? 2 : 3) void k_lora_up(LoraParams p) 
                 hl[s][2][lane] = lo;
             }
             __syncthreads();
-#pragma unroll
-            for (int s = 0; s < RS; ++s)
-#pragma unroll
-                for (int c = 0; c < 3; ++c) hp[s][c] = hl[s][c][lane];
         }
         for (int nb = nb0; nb < nb1; nb += UB) {
             const int n1 = min(16 * nb1, p.N);
             float* tile = sums[wv];
+            // (h's parts are read again for every UB blocks: 12 RS registers less, which
+            // would spill at rank 64)
+            asm volatile("" ::: "memory");
+            u32x4 hp[RS][3];
+#pragma unroll
+            for (int s = 0; s < RS; ++s)
+#pragma unroll
+                for (int c = 0; c < 3; ++c) hp[s][c] = hl[s][c][lane];
 #pragma unroll
             for (int u = 0; u < UB; ++u) {
                 f32x4 acc = {0, 0, 0, 0};
