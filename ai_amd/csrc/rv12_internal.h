@@ -244,7 +244,9 @@ struct AdjustParams {
     int32_t* pi = nullptr;
     int max_tokens, n_bias, slice;
 };
-// ids of one workgroup's slice: 4096, less while the rows are too few to fill the GPU
+// ids of one workgroup's slice: 4096, less while the rows are too few to fill the
+// GPU (151936 logits: one row 5.6 us in slices of 1024, 7.3 of 4096; 64 rows with
+// histories, biases and masks 24 us in slices of 4096, 34 of 1024, 28 of 8192)
 inline int adjust_slice(int64_t V, int T) {
     int s = 4096;
     while (s > 1024 && (V + s - 1) / s * T < 512) s /= 2;
@@ -277,15 +279,19 @@ constexpr int kMaxLoraRank = 128;
 // blocks of 16 ranks the kernels are built for: 1, 2, 4 or 8
 inline int lora_rank_blocks(int R) { return R <= 16 ? 1 : (R <= 32 ? 2 : (R <= 64 ? 4 : 8)); }
 // K splits of the first pass: 4 steps of 32 columns for each of its 4 waves, at
-// most 16 splits (the second pass adds them 16 lanes at a time)
+// most 16 splits (the second pass adds them 16 lanes at a time).  At 4096 columns, 16
+// rows of 13 adapters of rank 32: both passes 14.1 us in 8 splits, 15.6 in 4, 18.0
+// in 2, 13.7 in 16; 2051 rows of three of rank 64: 108, 112, 114, 117
 inline int lora_splits(int K) { return std::min((K / 32 + 15) / 16, 16); }
 // adapters of a tile side by side (the grid takes that many whether they are there
-// or not): all 16 while the tiles are few.  Blocks per wave of the second pass: as
-// many as leave 256 workgroups, which prepare the tile's h each (13 adapters, rank
-// 32, 6144 rows: 6.0 us with 4 blocks, 6.4 with 2 or 8, 10.1 with one)
+// or not): all 16 while the tiles are few (the 16 rows above: 80 us one after the
+// other, 31 with 4 side by side; the 2051 rows: 109 us one after the other, 116 with
+// 4, 176 with 16).  Blocks per wave of the second pass: as many as leave 256
+// workgroups, which prepare the tile's h each (the 16 rows beside 6144 outputs: 7.2
+// us with 4 blocks, 11.9 with one, 9.5 with 16)
 inline void lora_launch(LoraParams* p) {
     const int tiles = (p->T + 15) / 16, nblk = (p->N + 15) / 16;
-    p->slots = std::min(std::min(p->T, 16), std::max(1, 64 / tiles));
+    p->slots = std::min(std::min(p->T, 16), std::max(1, 128 / tiles));
     p->nbw = 16;
     while (p->nbw > 1 && (int64_t)((nblk + 4 * p->nbw - 1) / (4 * p->nbw)) * tiles * p->slots < 256) p->nbw /= 2;
 }

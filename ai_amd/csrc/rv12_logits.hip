@@ -10,6 +10,11 @@
 // that fall into the slice in LDS (integer adds and maxima: the order does not
 // matter), then passes over the slice once.  The history is read again by every
 // slice, 8 bytes a token from the L2, against 8 bytes per id from HBM.
+//
+// 64 rows of 151936 logits: 14.5 us without rules (the bytes' rate), 24 with
+// histories up to 6000 tokens, 32 biases, masks and the pick's first pass (the
+// barriers between clearing, counting and the pass, which eight workgroups a CU
+// overlap in part); the pick's second pass 4 us, a launch.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

@@ -12,6 +12,10 @@
 // slot 8 (l / 16) + 0..7 of lane l (the adapter's weights, 16 bytes a lane
 // straight from memory), B operand column l % 16 (the token), result rows
 // 4 (l / 16) + 0..3.
+//
+// A prompt is bound by y and out (2051 rows beside 24576 outputs, rank 64: 448 MB in
+// 15 + 93 us, 4.2 TB/s); a few rows by two launches of dependent round trips (4 + 5
+// us for one row, 7 + 7 for 16 of 13 adapters).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

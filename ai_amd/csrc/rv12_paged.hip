@@ -25,8 +25,9 @@ namespace rv12 {
 // position, q goes to q_out as float32, k and v into the row's page slot,
 // rounded once to the cache type.
 //
-// Bound by bytes (4 (H + 2 KV) HD read, 4 H HD + 2 KV HD EB written per row); at
-// a few rows by its latency.  HD / 8 lanes hold a head, 4 consecutive dims of
+// Bound by bytes (4 (H + 2 KV) HD read, 4 H HD + 2 KV HD EB written per row: 4099
+// rows of 32 heads over 8 into bf16 pages take 38 us, 4.9 TB/s, the rate of a copy);
+// at a few rows by its latency (2.5 us for one, 3.5 for 64).  HD / 8 lanes hold a head, 4 consecutive dims of
 // either rotation half each, so every access is 16 bytes (8 where bf16 is
 // stored) and the norm's sum stays within 16 lanes.  A workgroup of 256 threads
 // takes a share of one row's heads: the row's HD / 2 angles are computed once
@@ -169,6 +170,11 @@ void launch_paged_append(const PagedParams& p, hipStream_t st) {
 // maximum and sum, and join in LDS.  A row in one chunk is written at once; the
 // chunks of the others leave (sums, m, l) and k_paged_combine joins them in
 // chunk order.
+//
+// Bound by the cache's bytes once they are many: 64 rows of 500 to 8200 positions,
+// 32 heads over 8, bf16, 730 MB in 134 us (5.4 TB/s) and the join in 6; 32771
+// positions of one row 26 + 4 us.  A few short rows take 6 us of dependent
+// round trips (rows, table, keys, values, the join in LDS) and 3-4 us for the join.
 
 // the rows r = base + lane of a plan step: leader rows have the number of rows
 // they lead (nr) and the positions to cover (n, 0 for a padding row)
@@ -774,6 +780,10 @@ __global__ __launch_bounds__(kCombineThreads) void k_paged_combine(PagedParams p
 template <int HD, bool BF16>
 static void launch_paged_t(const PagedParams& p, hipStream_t st) {
     const dim3 grid((unsigned)(paged_items(p) * p.n_kv));
+    // no more rows than sequences: every bf16 key and value is read once, past the
+    // caches (64 rows of 500 to 8200 positions 140 -> 128-134 us).  Several rows of one
+    // sequence share them in the L2 (8 rows at 4104 positions: 17 us, 19 past it), and
+    // a float32 key row takes two loads of one line (the 64 rows: 278 us, 299 past it)
     if (BF16 && p.T <= p.n_seq) hipLaunchKernelGGL((k_paged_attend<HD, BF16, BF16>), grid, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((k_paged_attend<HD, BF16, false>), grid, dim3(256), 0, st, p);
     const int rows = paged_split_rows(p);
