@@ -58,12 +58,12 @@ class Head:
             adjust(self.logits[:T], ids=self.ids[:T], **rules)
             if temperature <= 0:
                 return self.ids[:T].tolist()
-            none = self.ids[:T].cpu().numpy() < 0
+            greedy = self.ids[:T].tolist()
         lg = self.logits[:T].cpu().numpy().astype(np.float64)
         out = []
         for t in range(T):
-            if rules and none[t]:
-                out.append(-1)
+            if rules and (greedy[t] < 0 or lg[t].max() == -np.inf):  # nothing allowed, or nothing likely
+                out.append(greedy[t])
                 continue
             z = (lg[t] - lg[t].max()) / temperature
             p = np.exp(z)

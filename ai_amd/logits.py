@@ -28,8 +28,8 @@ def _vector(t, name, dtype, T, dev):
 
 def adjust(x, out=None, tokens=None, length=None, prompt=None, penalties=None, bias_ids=None, bias=None, mask=None,
            ids=None):
-    """The rules on the logits x (float32 [T, V]) into out (None: in place), which
-    is returned.  Per row and id n, in float32 and this order:
+    """The rules on the logits x (float32 [T, V]) into out (None: in place; a given
+    out is x or does not overlap it), which is returned.  Per row and id n, in float32 and this order:
 
         n among the row's tokens:            l = l / repetition if l > 0 else l * repetition
         n generated c > 0 times:             l -= frequency * c + presence

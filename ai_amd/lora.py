@@ -54,7 +54,8 @@ class Adapters:
 
     @classmethod
     def from_pairs(cls, pairs, device="cuda"):
-        """From (A [r, K], B [N, r], alpha) of each adapter, ranks as they are."""
+        """From (A [r, K], B [N, r], alpha) of each adapter, ranks as they are; the
+        weights rounded to bf16, scale = alpha / r."""
         pairs = list(pairs)
         if not pairs:
             raise ValueError("Adapters: at least one adapter")
@@ -71,7 +72,7 @@ class Adapters:
 
     def apply(self, x, y, idx, mode=0, lnw=None, eps=1e-6, out=None):
         """out[t] = y[t] + scale B (A x'[t]) of adapter idx[t], for the T rows of
-        x; out None: into y.  mode, lnw and eps give x' as the shared linear's
+        x; out None: into y; a given out is y or does not overlap it.  mode, lnw and eps give x' as the shared linear's
         call has it (wcomp.gemvc1): modes 0 and 1 x' = x (float32 [T, K]), with
         lnw (bf16 [K]) its RMSNorm; mode 2 x' = silu(x[:, :K]) * x[:, K:].  idx:
         int32 [T], outside [0, count) (-1) no adapter: out[t] = y[t].  y and out:

@@ -430,7 +430,7 @@ typedef struct rv12_rules {
 } rv12_rules;
 
 /* y[r] = the rules on x[r], 1 <= t <= 65535 rows of 1 <= v < 2^31 - 65536 logits
- * (y may be x: each logit is read and written once).  ids: NULL, or int64[t] that
+ * (y may be x: each logit is read and written once; else the two do not overlap).  ids: NULL, or int64[t] that
  * receives the id of each row's largest y among the allowed ones, the smallest on
  * ties, NaN counting as larger than any number, -1 where the mask allows none.
  * ws: rv12_logits_workspace_bytes(v, t) bytes, 8-byte aligned, read only with ids.
@@ -458,7 +458,7 @@ typedef struct rv12_lora {
  * x (rows k floats apart, 2 k in mode 2) and x' as rv12_gemv: mode 0 or 1 x' = x,
  * with lnw the RMSNorm; mode 2 x' = silu(x[0:k]) * x[k:2k] (no lnw).  A row whose
  * idx is outside [0, count) has no adapter: out[i] = y[i].  out may be y (same
- * stride); strides in floats.  Products of x', a, b and the sums between are
+ * stride), else the two do not overlap; strides in floats.  Products of x', a, b and the sums between are
  * float32 exact to rounding (three bf16 parts), finite x assumed.  Two passes, no
  * atomics.  ws: rv12_lora_workspace_bytes(r, k, t) bytes, 16-byte aligned. */
 size_t rv12_lora_workspace_bytes(int r, int k, int t);

@@ -246,6 +246,13 @@ def test_head_pick_with_rules():
     assert head.pick(h, T, rules=rules) == [17, second, -1]
     got = head.pick(h, T, temperature=0.7, top_p=0.9, rng=np.random.default_rng(0), rules=rules)
     assert got[0] == 17 and got[1] != base[1] and got[2] == -1
+    # the ids that a mask allows all at -inf: the smallest of them, sampled too
+    words[2, 1] = 0b1010
+    rules["mask"] = torch.from_numpy(words).cuda()
+    rules["bias_ids"] = torch.tensor([[17, 17], [-1, -1], [33, 35]], device="cuda")
+    rules["bias"] = torch.tensor([[0.0, 100.0], [0.0, 0.0], [-np.inf, -np.inf]], device="cuda")
+    assert head.pick(h, T, rules=rules) == [17, second, 33]
+    assert head.pick(h, T, temperature=0.7, rng=np.random.default_rng(1), rules=rules)[2] == 33
     assert head.pick(h, T) == base
 
 
