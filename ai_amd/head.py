@@ -45,7 +45,9 @@ class Head:
         picks the most likely id, the smallest on ties.  rules: the keyword
         arguments of ai_amd.logits.adjust (tokens, length, prompt, penalties,
         bias_ids, bias, mask), applied to the logits before the pick; a row
-        whose mask allows no id gets -1."""
+        whose mask allows no id gets -1.  With rules a sampled row whose largest
+        logit is not finite (a bias of +inf, a NaN, allowed ids all at -inf)
+        gives the greedy id."""
         T = int(T)
         x = h[:T].float().contiguous()
         if temperature <= 0 and not rules:
@@ -62,10 +64,11 @@ class Head:
         lg = self.logits[:T].cpu().numpy().astype(np.float64)
         out = []
         for t in range(T):
-            if rules and (greedy[t] < 0 or lg[t].max() == -np.inf):  # nothing allowed, or nothing likely
+            top = lg[t].max()
+            if rules and not np.isfinite(top):  # no probabilities to draw by
                 out.append(greedy[t])
                 continue
-            z = (lg[t] - lg[t].max()) / temperature
+            z = (lg[t] - top) / temperature
             p = np.exp(z)
             p /= p.sum()
             o = np.argsort(-p, kind="stable")

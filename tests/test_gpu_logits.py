@@ -256,6 +256,28 @@ def test_head_pick_with_rules():
     assert head.pick(h, T) == base
 
 
+def test_head_pick_sampled_beside_infinite_logits():
+    """A bias of +inf forces its id (the smallest of several), sampled too, and a
+    NaN logit gives its id, as in the greedy pick; the rows beside keep the draws
+    that they have alone."""
+    from ai_amd.head import Head
+    g = torch.Generator(device="cuda").manual_seed(9)
+    V, D, T = 3000, 256, 4
+    W = (torch.randn(V, D, device="cuda", generator=g) * 0.05).bfloat16()
+    h = torch.randn(T, D, device="cuda", generator=g)
+    head = Head(W)
+    inf = float("inf")
+    rules = {"bias_ids": torch.tensor([[2001, 77], [-1, -1], [5, 9], [8, 1500]], device="cuda"),
+             "bias": torch.tensor([[inf, inf], [0.0, 0.0], [inf, -inf], [1.0, float("nan")]], device="cuda")}
+    greedy = head.pick(h, T, rules=rules)
+    base = head.pick(h, T)
+    assert greedy == [77, base[1], 5, 1500]
+    alone = {k: v[1:2].contiguous() for k, v in rules.items()}
+    want = head.pick(h[1:2], 1, temperature=2.0, rng=np.random.default_rng(3), rules=alone)
+    got = head.pick(h, T, temperature=2.0, rng=np.random.default_rng(3), rules=rules)
+    assert got == [77, want[0], 5, 1500]
+
+
 def test_refusals():
     from ai_amd import logits
     T, V = 2, 100
