@@ -20,6 +20,8 @@ import torch
 from . import wcomp
 from .logits import adjust
 
+RULES = {"tokens", "length", "prompt", "penalties", "bias_ids", "bias", "mask"}  # adjust's inputs
+
 
 class Head:
     def __init__(self, Wu16, TM=16, device="cuda"):
@@ -48,6 +50,8 @@ class Head:
         whose mask allows no id gets -1.  With rules a sampled row whose largest
         logit is not finite (a bias of +inf, a NaN, allowed ids all at -inf)
         gives the greedy id."""
+        if rules and not RULES.issuperset(rules):
+            raise ValueError("pick: rules may hold " + ", ".join(sorted(RULES)))
         T = int(T)
         x = h[:T].float().contiguous()
         if temperature <= 0 and not rules:

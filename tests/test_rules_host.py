@@ -76,3 +76,16 @@ def test_cpu_tensors_are_refused():
         logits.adjust(torch.zeros(1, 8))
     with pytest.raises(ValueError):
         Adapters(torch.zeros(1, 8, 32, dtype=torch.bfloat16), torch.zeros(1, 4, 8, dtype=torch.bfloat16), torch.zeros(1))
+
+
+def test_head_pick_refuses_outputs_among_the_rules():
+    """The rules that Head.pick passes on are inputs: logits sent elsewhere would
+    leave a sampled pick without the rules."""
+    from ai_amd.head import Head
+    head = Head.__new__(Head)  # refused before the head's matrix is looked at
+    h = torch.zeros(1, 8)
+    for rules in ({"out": torch.zeros(1, 100)}, {"ids": torch.zeros(1, dtype=torch.int64)}, {"x": h},
+                  {"mask": None, "out": None}, {"penalty": None}):
+        for temperature in (0.0, 1.0):
+            with pytest.raises(ValueError, match="rules"):
+                head.pick(h, 1, temperature=temperature, rules=rules)
