@@ -26,12 +26,13 @@ namespace rv12 {
 // rounded once to the cache type.
 //
 // Bound by bytes (4 (H + 2 KV) HD read, 4 H HD + 2 KV HD EB written per row: 4099
-// rows of 32 heads over 8 into bf16 pages take 38 us, 4.9 TB/s, the rate of a copy);
-// at a few rows by its latency (2.5 us for one, 3.5 for 64).  HD / 8 lanes hold a head, 4 consecutive dims of
-// either rotation half each, so every access is 16 bytes (8 where bf16 is
-// stored) and the norm's sum stays within 16 lanes.  A workgroup of 256 threads
-// takes a share of one row's heads: the row's HD / 2 angles are computed once
-// per workgroup, while the heads' loads are in flight.
+// rows of 32 heads over 8 take 37 us into bf16 pages, 5.0 TB/s, and 42 into float32
+// ones, 4.8: the rate of a copy); at a few rows by its latency (2.5 us for one, 3.5
+// for 64).  HD / 8 lanes hold a head, 4 consecutive dims of either rotation half
+// each, so every access is 16 bytes (8 where bf16 is stored) and the norm's sum
+// stays within 16 lanes.  A workgroup of 256 threads takes a share of one row's
+// heads: the row's HD / 2 angles are computed once per workgroup, while the heads'
+// loads are in flight.
 //
 // The angle pos inv[i] passes 2^24 turns' worth of float32 steps in a long
 // context (its float32 product is off by 0.004 rad at position 120000), so it
@@ -43,20 +44,20 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedParams p) {
     __shared__ float2 cs[half];                 // (cos, sin) of the row's angles
     const int r = blockIdx.x, t = threadIdx.x;
     const int H = p.n_heads, KV = p.n_kv, NH = H + 2 * KV;
-    const int slots = 256 / LPH;  // heads at once
+    const int slots = 256 / LPH;  // heads of a workgroup
     const int hl = t % LPH;       // the lane's dims: 4 hl .. + 3 of both halves
     const int64_t sq = p.seq ? (int64_t)p.seq[r] : r;
     const int64_t pos = p.pos[r];
     const bool live = sq >= 0 && sq < p.n_seq && pos >= 0 && pos < p.cap;
     const float* row = p.qkv + (int64_t)r * NH * HD;
-    int h = blockIdx.y * slots + t / LPH;
+    const int h = blockIdx.y * slots + t / LPH;
     f32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
     if (h < NH) {
         a = *reinterpret_cast<const f32x4*>(row + (int64_t)h * HD + 4 * hl);
         b = *reinterpret_cast<const f32x4*>(row + (int64_t)h * HD + half + 4 * hl);
     }
     if (!live) {
-        for (; h < H; h += slots * gridDim.y) {
+        if (h < H) {
             float* dst = p.qo + ((int64_t)r * H + h) * HD;
             *reinterpret_cast<f32x4*>(dst + 4 * hl) = f32x4{0, 0, 0, 0};
             *reinterpret_cast<f32x4*>(dst + half + 4 * hl) = f32x4{0, 0, 0, 0};
@@ -76,58 +77,51 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedParams p) {
     const bool paged = pid >= 0 && pid < p.n_pages;
     const int64_t slot = ((paged ? pid : 0) * KV << p.page_log) + (pos & ((1 << p.page_log) - 1));
     __syncthreads();
-    for (; h < NH; h += slots * gridDim.y) {
-        f32x4 o0 = a, o1 = b;
-        if (h < H + KV) {
-            const float* nw = h < H ? p.qn : p.kn;
-            const f32x4 wa = *reinterpret_cast<const f32x4*>(nw + 4 * hl);
-            const f32x4 wb = *reinterpret_cast<const f32x4*>(nw + half + 4 * hl);
-            float s = 0.0f;
+    if (h >= NH) return;
+    if (h < H + KV) {
+        const float* nw = h < H ? p.qn : p.kn;
+        const f32x4 wa = *reinterpret_cast<const f32x4*>(nw + 4 * hl);
+        const f32x4 wb = *reinterpret_cast<const f32x4*>(nw + half + 4 * hl);
+        float s = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s = fmaf(a[e], a[e], fmaf(b[e], b[e], s));
-            s += dpp<kDppXor1>(s);
-            s += dpp<kDppXor2>(s);
-            s += dpp<kDppHalfMirror>(s);
-            if constexpr (LPH == 16) s += dpp<kDppMirror>(s);
-            const float rs = 1.0f / sqrtf(s / (float)HD + p.eps);
+        for (int e = 0; e < 4; ++e) s = fmaf(a[e], a[e], fmaf(b[e], b[e], s));
+        s += dpp<kDppXor1>(s);
+        s += dpp<kDppXor2>(s);
+        s += dpp<kDppHalfMirror>(s);
+        if constexpr (LPH == 16) s += dpp<kDppMirror>(s);
+        const float rs = 1.0f / sqrtf(s / (float)HD + p.eps);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 c = cs[4 * hl + e];
-                const float x = wa[e] * (a[e] * rs), y = wb[e] * (b[e] * rs);
-                o0[e] = x * c.x - y * c.y;
-                o1[e] = y * c.x + x * c.y;
-            }
+        for (int e = 0; e < 4; ++e) {
+            const float2 c = cs[4 * hl + e];
+            const float x = wa[e] * (a[e] * rs), y = wb[e] * (b[e] * rs);
+            a[e] = x * c.x - y * c.y;
+            b[e] = y * c.x + x * c.y;
         }
-        const int hn = h + slots * gridDim.y;
-        if (hn < NH) {
-            a = *reinterpret_cast<const f32x4*>(row + (int64_t)hn * HD + 4 * hl);
-            b = *reinterpret_cast<const f32x4*>(row + (int64_t)hn * HD + half + 4 * hl);
-        }
-        if (h < H) {
-            float* dst = p.qo + ((int64_t)r * H + h) * HD;
-            *reinterpret_cast<f32x4*>(dst + 4 * hl) = o0;
-            *reinterpret_cast<f32x4*>(dst + half + 4 * hl) = o1;
-        } else if (paged) {
-            const int g = h < H + KV ? h - H : h - H - KV;
-            void* c = h < H + KV ? p.kc : p.vc;
-            const int64_t off = (slot + ((int64_t)g << p.page_log)) * HD + 4 * hl;
-            if constexpr (BF16) {
-                uint16_t* dst = static_cast<uint16_t*>(c) + off;
-                *reinterpret_cast<uint2*>(dst) =
-                    uint2{bf16_bits(o0[0]) | bf16_bits(o0[1]) << 16, bf16_bits(o0[2]) | bf16_bits(o0[3]) << 16};
-                *reinterpret_cast<uint2*>(dst + half) =
-                    uint2{bf16_bits(o1[0]) | bf16_bits(o1[1]) << 16, bf16_bits(o1[2]) | bf16_bits(o1[3]) << 16};
-            } else {
-                float* dst = static_cast<float*>(c) + off;
-                *reinterpret_cast<f32x4*>(dst) = o0;
-                *reinterpret_cast<f32x4*>(dst + half) = o1;
-            }
+    }
+    if (h < H) {
+        float* dst = p.qo + ((int64_t)r * H + h) * HD;
+        *reinterpret_cast<f32x4*>(dst + 4 * hl) = a;
+        *reinterpret_cast<f32x4*>(dst + half + 4 * hl) = b;
+    } else if (paged) {
+        const int g = h < H + KV ? h - H : h - H - KV;
+        void* c = h < H + KV ? p.kc : p.vc;
+        const int64_t off = (slot + ((int64_t)g << p.page_log)) * HD + 4 * hl;
+        if constexpr (BF16) {
+            uint16_t* dst = static_cast<uint16_t*>(c) + off;
+            *reinterpret_cast<uint2*>(dst) =
+                uint2{bf16_bits(a[0]) | bf16_bits(a[1]) << 16, bf16_bits(a[2]) | bf16_bits(a[3]) << 16};
+            *reinterpret_cast<uint2*>(dst + half) =
+                uint2{bf16_bits(b[0]) | bf16_bits(b[1]) << 16, bf16_bits(b[2]) | bf16_bits(b[3]) << 16};
+        } else {
+            float* dst = static_cast<float*>(c) + off;
+            *reinterpret_cast<f32x4*>(dst) = a;
+            *reinterpret_cast<f32x4*>(dst + half) = b;
         }
     }
 }
 
 void launch_paged_append(const PagedParams& p, hipStream_t st) {
-    // every head of a row at once
+    // a row's heads in one or more workgroups, a head each for its LPH threads
     const int slots = 256 / (p.head_dim / 8), nh = p.n_heads + 2 * p.n_kv;
     const dim3 grid((unsigned)p.T, (unsigned)((nh + slots - 1) / slots));
     if (p.head_dim == 128) {
