@@ -177,7 +177,7 @@ struct PlanItem {
     int C;              // chunk length
     int chunk, chunks;  // of this row
     int slot;           // first partial of the row (rows of several chunks only)
-    int unused;
+    int once;           // no row before or after these is of their sequence
 };
 struct PagedParams {
     const float* qkv = nullptr;

@@ -171,10 +171,11 @@ void launch_paged_append(const PagedParams& p, hipStream_t st) {
 // round trips (rows, table, keys, values, the join in LDS) and 3-4 us for the join.
 
 // the rows r = base + lane of a plan step: leader rows have the number of rows
-// they lead (nr) and the positions to cover (n, 0 for a padding row)
+// they lead (nr) and the positions to cover (n, 0 for a padding row); key: the row's
+// sequence, another negative number for every row without one
 struct PlanRows {
     bool leader;
-    int nr, n;
+    int nr, n, key;
 };
 
 template <int CTRL, int ROWS = 0xF>
@@ -213,6 +214,7 @@ __device__ __forceinline__ PlanRows plan_rows(const PagedParams& p, int base) {
     o.leader = r < p.T && !joins;
     o.nr = 1;
     o.n = n;
+    o.key = key;
     if (m) {
         o.nr = 1 + __builtin_ctzll(~((m >> lane) >> 1));
         int k;
@@ -272,6 +274,9 @@ __device__ __forceinline__ bool plan_find(const PagedParams& p, int want, PlanIt
     it->chunk = want - __builtin_amdgcn_readlane(e, s);
     it->chunks = __builtin_amdgcn_readlane(ch, s);
     it->slot = __builtin_amdgcn_readlane((both >> 16) - sl, s);
+    const int key = __builtin_amdgcn_readlane(o.key, s), e1 = s + it->nr;
+    it->once = !((s > 0 && __builtin_amdgcn_readlane(o.key, max(s - 1, 0)) == key) ||
+                 (e1 < p.T && __builtin_amdgcn_readlane(o.key, min(e1, 63)) == key));
     return true;
 }
 
@@ -334,7 +339,11 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PagedParams p) {
         it.chunks = ch;
         it.slot = slots + le - sl;
         it.chunk = 0;
-        it.unused = 0;
+        it.once = 1;
+        if (p.seq && o.leader && o.key >= 0) {
+            const int r0 = it.row, r1 = it.row + it.nr;
+            it.once = !((r0 > 0 && p.seq[r0 - 1] == o.key) || (r1 < p.T && p.seq[r1] == o.key));
+        }
         if (se) p.plan[1 + p.plan_items + rows + re - 1] = it;
         for (int i = 0; i < ch; ++i) {
             it.chunk = i;
@@ -376,8 +385,15 @@ __device__ __forceinline__ float* paged_part(const PagedParams& p, int HD, int s
     return p.part + ((int64_t)slot * p.n_kv + g) * (p.rt * p.g) * (HD + 4);
 }
 
+template <int HD, bool BF16>
+struct AttendLds {
+    float part[4 * (HD / 16 * 256 + 128)];
+    u32x4 qp[BF16 ? HD / 32 : 1][3][BF16 ? 64 : 1];
+    f32x4 qf[BF16 ? 1 : HD / 32][2][BF16 ? 1 : 64];
+};
+
 template <int HD, bool BF16, bool ONCE>
-__global__ __launch_bounds__(256, 3) void k_paged_attend(PagedParams p) {
+__device__ __forceinline__ void attend_item(const PagedParams& p, const PlanItem& it, AttendLds<HD, BF16>& sh) {
     constexpr int EB = BF16 ? 2 : 4;   // cache bytes per value
     constexpr int NB = BF16 ? 2 : 1;   // blocks of 16 positions per step
     constexpr int PB = 16 * NB;
@@ -388,25 +404,14 @@ __global__ __launch_bounds__(256, 3) void k_paged_attend(PagedParams p) {
     constexpr int NW = 4;              // waves
     constexpr int ROWB = HD * EB;      // bytes of one position
     constexpr int kPolicy = ONCE ? kNonTemporal : 0;
-    __shared__ float lds[NW * (DT * 256 + 128)];
-    __shared__ u32x4 qp[BF16 ? NA : 1][3][BF16 ? 64 : 1];
-    __shared__ f32x4 qf[BF16 ? 1 : NA][2][BF16 ? 1 : 64];
+    float* lds = sh.part;
+    auto& qp = sh.qp;
+    auto& qf = sh.qf;
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q4 = lane >> 4, c16 = lane & 15;
-    const int g = blockIdx.x % p.n_kv, item = blockIdx.x / p.n_kv;
+    const int g = blockIdx.x % p.n_kv;
     const int G = p.g, H = p.n_heads;
-
-    PlanItem it;
-    if (!plan_find<false>(p, item, &it)) return;
-    // (said to be uniform, so that the loads' descriptors stay in scalar registers)
-    it.row = __builtin_amdgcn_readfirstlane(it.row);
-    it.nr = __builtin_amdgcn_readfirstlane(it.nr);
-    it.n = __builtin_amdgcn_readfirstlane(it.n);
-    it.C = __builtin_amdgcn_readfirstlane(it.C);
-    it.chunk = __builtin_amdgcn_readfirstlane(it.chunk);
-    it.chunks = __builtin_amdgcn_readfirstlane(it.chunks);
-    it.slot = __builtin_amdgcn_readfirstlane(it.slot);
 
     // this lane's column: head cg of row r0 + rt
     const int rt = c16 / G, cg = c16 - rt * G;
@@ -716,6 +721,35 @@ __global__ __launch_bounds__(256, 3) void k_paged_attend(PagedParams p) {
     if (!whole && wv == 0 && q4 == 0) *reinterpret_cast<float2*>(part + HD) = float2{mj, lj};
 }
 
+// Loads past the caches: where the item's rows have their sequence to themselves
+// (the rows before and after them are of others), every key and value of bf16 caches
+// is read once and the loads stream: a pass over a model's layers comes back to a
+// layer's keys when the other layers' have gone by.  Both passes, 32 heads over 8, us
+// streaming and through the caches: 8 rows at 1000 positions 15.1, 16.2; 24 at 4100
+// 78, 85; 64 at 8200 344, 385.  (Keys still in the 256 MB cache from a call just
+// before are the exception: 8 rows at 4100 36.8, 31.6.)  Items that share a sequence
+// find its keys in the L2 (64 heads over 8, 8 rows at 4104 positions: 21.7, 22.6 past
+// it), and a float32 key row takes two loads of one line (64 rows of 500 to 8200
+// positions: 278, 299 past it).  The policy is a part of the instructions, so bf16 has
+// the body twice, chosen before anything of it is issued: chosen inside it, the waits
+// of both merged (142 -> 146 us for the 64 rows in bf16).
+template <int HD, bool BF16>
+__global__ __launch_bounds__(256, 3) void k_paged_attend(PagedParams p) {
+    __shared__ AttendLds<HD, BF16> sh;
+    PlanItem it;
+    if (!plan_find<false>(p, blockIdx.x / p.n_kv, &it)) return;
+    // (said to be uniform, so that the loads' descriptors stay in scalar registers)
+    it.row = __builtin_amdgcn_readfirstlane(it.row);
+    it.nr = __builtin_amdgcn_readfirstlane(it.nr);
+    it.n = __builtin_amdgcn_readfirstlane(it.n);
+    it.C = __builtin_amdgcn_readfirstlane(it.C);
+    it.chunk = __builtin_amdgcn_readfirstlane(it.chunk);
+    it.chunks = __builtin_amdgcn_readfirstlane(it.chunks);
+    it.slot = __builtin_amdgcn_readfirstlane(it.slot);
+    if (BF16 && __builtin_amdgcn_readfirstlane(it.once)) attend_item<HD, BF16, BF16>(p, it, sh);
+    else attend_item<HD, BF16, false>(p, it, sh);
+}
+
 // joins the chunks of the rows that have several: out = sum 2^(m_c - M) acc_c /
 // sum 2^(m_c - M) l_c.  Workgroup (row among them, kv head, query head of it); HD /
 // 4 threads hold a head's dims, the chunks go round the groups of threads, each
@@ -774,12 +808,7 @@ __global__ __launch_bounds__(kCombineThreads) void k_paged_combine(PagedParams p
 template <int HD, bool BF16>
 static void launch_paged_t(const PagedParams& p, hipStream_t st) {
     const dim3 grid((unsigned)(paged_items(p) * p.n_kv));
-    // no more rows than sequences: every bf16 key and value is read once, past the
-    // caches (64 rows of 500 to 8200 positions 140 -> 128-134 us).  Several rows of one
-    // sequence share them in the L2 (8 rows at 4104 positions: 17 us, 19 past it), and
-    // a float32 key row takes two loads of one line (the 64 rows: 278 us, 299 past it)
-    if (BF16 && p.T <= p.n_seq) hipLaunchKernelGGL((k_paged_attend<HD, BF16, BF16>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((k_paged_attend<HD, BF16, false>), grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((k_paged_attend<HD, BF16>), grid, dim3(256), 0, st, p);
     const int rows = paged_split_rows(p);
     if (rows)
         hipLaunchKernelGGL((k_paged_combine<HD>), dim3((unsigned)rows, (unsigned)p.n_kv, (unsigned)p.g),

@@ -455,3 +455,32 @@ def test_attend_prompt_behind_a_long_context(kv):
         b = torch.empty_like(a)
         p.attend(q, seq, pos, table, kc, vc, b)
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("H,KV,HD", [(32, 8, 128), (64, 8, 128), (44, 4, 128), (8, 4, 64), (7, 7, 64)])
+@pytest.mark.parametrize("kv", KV_TYPES)
+def test_attend_does_not_depend_on_the_table_height(H, KV, HD, kv):
+    """Rows with a sequence of their own, runs of one sequence (within a tile of
+    rows, over its end, at the pass's ends) and padding in one pass: right, and the
+    same bits with more rows in the table than the pass has."""
+    from ai_amd.attn import PagedRopeAttn
+    page = 16
+    g = _gen(H, KV, HD, 11)
+    lens = [700, 33, 1040, 90, 260]
+    print("case", H, KV, HD, kv, flush=True)
+    table, n_pages = _table(lens, page, g)
+    tall = torch.full((64, table.shape[1]), -1, dtype=torch.int32, device="cuda")
+    tall[:len(lens)] = table
+    kc, vc = _randn(g, n_pages, KV, page, HD).to(kv), _randn(g, n_pages, KV, page, HD).to(kv)
+    p = PagedRopeAttn(H, KV, HD, page, kv, EPS)
+    runs = [[(0, 698), (0, 699), (1, 32), (2, 1039), (-1, 0), (3, 87), (3, 88), (3, 89), (4, 259), (2, 1038)],
+            [(0, j) for j in range(688, 700)], [(1, 5), (0, 699), (0, 698), (0, 697), (0, 696)],
+            [(i % 5, lens[i % 5] - 1 - i // 5) for i in range(75)]]
+    for rows in runs:
+        seq = torch.tensor([r[0] for r in rows], dtype=torch.int32, device="cuda")
+        pos = torch.tensor([r[1] for r in rows], device="cuda")
+        q = _randn(g, len(rows), H * HD) * 2
+        a = _check(p, q, seq, pos, table, kc, vc)
+        b = torch.full_like(a, float("nan"))
+        p.attend(q, seq, pos, tall, kc, vc, b)
+        assert torch.equal(a, b)
