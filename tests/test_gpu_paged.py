@@ -484,3 +484,114 @@ def test_attend_does_not_depend_on_the_table_height(H, KV, HD, kv):
         b = torch.full_like(a, float("nan"))
         p.attend(q, seq, pos, tall, kc, vc, b)
         assert torch.equal(a, b)
+
+
+def _plan_of(seq, lens, n_kv, G, bf16):
+    """(chunk length, chunks of each leader) of a pass without padding: rows of one
+    sequence next to each other within an aligned tile share their chunks."""
+    from test_paged_host import _plan
+    rt = 1
+    while 2 * rt * G <= 16:
+        rt *= 2
+    lead = []
+    for r, (s, n) in enumerate(zip(seq, lens)):
+        if r % rt and s == seq[r - 1]:
+            lead[-1] = max(lead[-1], n)
+        else:
+            lead.append(n)
+    return _plan(lead, n_kv, 128 if bf16 else 64)
+
+
+def _block_values(g, n_pages, KV, page, HD, kv):
+    """Keys and values whose every block of 16 positions shows in the output: small
+    keys, so that all positions weigh about the same, and values of -1 or 1, one sign
+    per block and dim."""
+    kc = (_randn(g, n_pages, KV, page, HD) * 0.05).to(kv)
+    sign = torch.randint(0, 2, (n_pages, KV, page // 16, 1, HD), generator=g, device="cuda") * 2 - 1
+    return kc, sign.expand(-1, -1, -1, 16, -1).reshape(n_pages, KV, page, HD).to(kv).contiguous()
+
+
+def _check_blocks(p, q, seq, pos, table, kc, vc, C, chunks):
+    """The attention within a bound by the plan's chunk length (112 roundings per 128
+    positions of a chunk, one per chunk), which the output without any one block of
+    a row would exceed."""
+    H, KV, HD, page, G = p.n_heads, p.n_kv, p.head_dim, p.page, p.n_heads // p.n_kv
+    out = torch.full_like(q, float("nan"))
+    p.attend(q, seq, pos, table, kc, vc, out)
+    torch.cuda.synchronize()
+    worst, least = 0.0, 1e9
+    for r, (s, n) in enumerate(zip(seq.tolist(), (pos + 1).tolist())):
+        ids = table[s, :-(-n // page)].long()
+        K, V = (c[ids.clamp(min=0)].double().transpose(0, 1).reshape(KV, -1, HD)[:, :n].contiguous() for c in (kc, vc))
+        z = torch.matmul(q[r].double().view(KV, G, HD), K.transpose(1, 2).contiguous()) * HD ** -0.5
+        zabs = torch.matmul(q[r].double().view(KV, G, HD).abs(), K.abs().transpose(1, 2).contiguous()) * HD ** -0.5
+        gone = (ids < 0).repeat_interleave(page)[:n]
+        w = torch.softmax(z.masked_fill(gone, -math.inf), -1)
+        ref = torch.matmul(w, V)
+        delta = (HD + 4) * U * zabs.amax(-1, keepdim=True)
+        rel = 4 * delta + 2.0 ** -21 + (112 * max(1, min(C, n) / 128) + chunks + 64) * U
+        bound = rel * torch.matmul(w, V.abs())
+        err = (out[r].double().view_as(ref) - ref).abs()
+        assert bool((err <= bound).all()), (r, float((err / bound).max()))
+        # without block b: the output moves by w_b / (1 - w_b) (out - V_b)
+        m = n // 16 * 16
+        wb = w[..., :m].reshape(KV, G, -1, 16).sum(-1)
+        vb = V[:, :m].reshape(KV, -1, 16, HD)[:, :, 0]
+        there = ~gone[:m:16]
+        move = (wb / (1 - wb))[..., None] * (ref[:, :, None] - vb[:, None]).abs()
+        move = (move / bound[:, :, None]).amax((0, 1, 3))[there]
+        worst, least = max(worst, float((err / bound).max())), min(least, float(move.min()))
+    assert least > 2, least
+    return worst, least
+
+
+@pytest.mark.parametrize("H,KV,HD", [(8, 8, 64), (64, 8, 128)])
+@pytest.mark.parametrize("kv", KV_TYPES)
+@pytest.mark.parametrize("rows", ["alone", "pairs", "apart"])
+def test_attend_long_chunks(H, KV, HD, kv, rows):
+    """Chunks of more than 4096 positions, past the 64 blocks whose page ids a wave
+    loads at once: new tokens of 64 sequences, two tokens each of 64 (the plan of more
+    than 64 rows), and pairs of rows whose limits lie apart from before that place
+    on.  Pages are missing on both sides of it, in other places in every sequence."""
+    from ai_amd.attn import PagedRopeAttn
+    page, n = 16, 9003
+    g = _gen(H, HD, 12, rows == "alone", rows == "apart")
+    print("case", H, KV, HD, kv, rows, flush=True)
+    one, n_pages = _table([n], page, g)
+    kc, vc = _block_values(g, n_pages, KV, page, HD, kv)
+    table = one.repeat(64, 1)  # the sequences share their pages
+    if rows == "alone":
+        at = [(i, n - 1 - i) for i in range(64)]
+    else:
+        at = [(i, p) for i in range(64) for p in ((n - 2, n - 1) if rows == "pairs" else (3000 + i, n - 1 - i))]
+    seq = torch.tensor([a[0] for a in at], dtype=torch.int32, device="cuda")
+    pos = torch.tensor([a[1] for a in at], device="cuda")
+    C, chunks = _plan_of([a[0] for a in at], [a[1] + 1 for a in at], KV, H // KV, kv == torch.bfloat16)
+    assert 4096 + 256 <= C < 4700 and max(chunks) == 2
+    for i in range(64):
+        for c0 in (0, C):  # blocks 4096 positions into each chunk, by 16 positions on either side
+            first = (c0 + 4096) // page
+            near = torch.randperm(16, generator=g, device="cuda")[:5] - 8 + first
+            table[i, near[near < one.shape[1]]] = -1
+    q = _randn(g, len(at), H * HD)
+    p = PagedRopeAttn(H, KV, HD, page, kv, EPS)
+    print(_check_blocks(p, q, seq, pos, table, kc, vc, C, max(chunks)), flush=True)
+
+
+@pytest.mark.parametrize("kv", KV_TYPES)
+def test_long_context_leaves_no_block_out(kv):
+    """A 30000-position sequence in many chunks beside short ones, under a bound that
+    one block of 16 positions too few exceeds."""
+    from ai_amd.attn import PagedRopeAttn
+    H, KV, HD, page = 32, 8, 128, 64
+    g = _gen(13)
+    lens = [30000] + [100 + 37 * i for i in range(40)]
+    table, n_pages = _table(lens, page, g)
+    kc, vc = _block_values(g, n_pages, KV, page, HD, kv)
+    seq = torch.arange(len(lens), dtype=torch.int32, device="cuda")
+    pos = torch.tensor([n - 1 for n in lens], device="cuda")
+    C, chunks = _plan_of(list(range(len(lens))), lens, KV, H // KV, kv == torch.bfloat16)
+    assert chunks[0] > 20
+    q = _randn(g, len(lens), H * HD)
+    p = PagedRopeAttn(H, KV, HD, page, kv, EPS)
+    print(_check_blocks(p, q, seq, pos, table, kc, vc, C, max(chunks)), flush=True)
