@@ -131,7 +131,8 @@ class PagedRopeAttn:
     A row with seq or pos outside the table (-1 for padding a pass to a fixed
     size) is padding: its q and out are zeros and it writes nothing.  A page id
     outside the cache (-1) is no page: its positions take no part in the
-    attention, a key or value for it is dropped.  Rows that name one slot
+    attention, a key or value for it is dropped.  A row that sees an infinite key
+    or value may be NaN.  Rows that name one slot
     together leave it with either's key and value.  seq, pos and table are read
     on the device, so a call can be captured in a HIP graph; every call has a
     workspace of its own.  The rotation angle is formed in 64 bits (RopeAttn's

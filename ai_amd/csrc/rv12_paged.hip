@@ -157,8 +157,8 @@ void launch_paged_append(const PagedParams& p, hipStream_t st) {
 // bf16 caches: exact products on the bf16 matrix cores with q and the
 // probabilities split into three bf16 parts (24 bits), 32 positions per value
 // product; float32 caches: the float32 matrix cores.  Sums, maxima and the
-// running rescale are float32.  (An infinite cache value gives NaN, as a part of
-// 0 meets it.)
+// running rescale are float32.  (An infinite value of a bf16 cache gives NaN where a
+// part of 0 meets it; a float32 one gives what its product does.)
 //
 // The four waves of a workgroup take blocks in turn, each with its own running
 // maximum and sum, and join in LDS.  A row in one chunk is written at once; the

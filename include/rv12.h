@@ -391,13 +391,15 @@ int rv12_paged_append(const rv12_paged* a, int t, const float* qkv, const float*
  * positions, the rows' own among them, are in the cache before the call.
  * Positions without a page take no part; a row that is padding, or has nothing
  * left to attend, gives zeros.  Slots past a row's position are not read into it,
- * whatever they hold; an infinite key or value that it sees gives NaN.  The chunks of
- * positions, about 1024 workgroups whatever the lengths, and so a result's last bits
- * depend on the lengths of all rows.  Two passes (the chunks; the join of the rows
- * in several, in chunk order), before them for more than 64 rows a small one that
- * lists the chunks; no atomics.  ws: rv12_paged_attend_workspace_bytes(a, t) bytes, 16-byte aligned
- * (0 bytes there: a or t out of range); calls that overlap need their own.  The
- * paged counterpart of rope_attn_k's and attn_k's attention,
+ * whatever they hold.  An infinite key or value that it sees gives NaN or the
+ * value's infinity; of a float32 cache a score of -inf weighs nothing, and a row
+ * whose scores are all -inf gives zeros or NaN.  The chunks of positions, about
+ * 1024 workgroups whatever the lengths, and so a result's last bits depend on the
+ * lengths of all rows.  Two passes (the chunks; the join of the rows in several, in
+ * chunk order), before them for more than 64 rows a small one that lists the
+ * chunks; no atomics.  ws: rv12_paged_attend_workspace_bytes(a, t) bytes, 16-byte
+ * aligned (0 bytes there: a or t out of range); calls that overlap need their own.
+ * The paged counterpart of rope_attn_k's and attn_k's attention,
  * ramvi/engine/ramvi_engine/kernels/tkernels.py:123-213. */
 size_t rv12_paged_attend_workspace_bytes(const rv12_paged* a, int t);
 int rv12_paged_attend(const rv12_paged* a, int t, const float* q, const int32_t* seq, const int64_t* pos,

@@ -595,3 +595,29 @@ def test_long_context_leaves_no_block_out(kv):
     q = _randn(g, len(lens), H * HD)
     p = PagedRopeAttn(H, KV, HD, page, kv, EPS)
     print(_check_blocks(p, q, seq, pos, table, kc, vc, C, max(chunks)), flush=True)
+
+
+@pytest.mark.parametrize("kv", KV_TYPES)
+def test_attend_infinite_keys_and_values(kv):
+    """A row that sees an infinite key or value: NaN, an infinity of the value's sign,
+    or zeros where every score is -inf.  Every element is written, and the rows beside
+    are not touched."""
+    from ai_amd.attn import PagedRopeAttn
+    H, KV, HD, page = 32, 8, 128, 16
+    g = _gen(14)
+    lens = [600, 40, 16, 20]
+    table, n_pages = _table(lens, page, g)
+    kc, vc = _randn(g, n_pages, KV, page, HD).to(kv), _randn(g, n_pages, KV, page, HD).to(kv)
+    pos = torch.tensor([n - 1 for n in lens], device="cuda")
+    q = _randn(g, len(lens), H * HD) * 2
+    q[2] = 1.0
+    p = PagedRopeAttn(H, KV, HD, page, kv, EPS)
+    out = _check(p, q, None, pos, table, kc, vc)
+    kc[int(table[2, 0])] = -float("inf")  # every score of row 2
+    vc[int(table[3, 0]), :, 5] = float("inf")
+    o2 = torch.full_like(out, 7.0)
+    p.attend(q, None, pos, table, kc, vc, o2)
+    torch.cuda.synchronize()
+    assert torch.equal(o2[:2], out[:2])
+    assert bool((o2[2].isnan() | (o2[2] == 0)).all())
+    assert bool((o2[3].isnan() | (o2[3] == float("inf"))).all())
