@@ -210,11 +210,15 @@ constexpr int kPagedInlineRows = 64;
 inline int64_t paged_items(const PagedParams& p) {
     return std::min((int64_t)p.target / p.n_kv + p.T, (int64_t)p.T * ((p.cap + p.grain - 1) / p.grain));
 }
-// rows of several chunks at most (n > C each), and their chunks (fewer than 2 n / C each)
+// rows of several chunks at most (n > C each), and their chunks (fewer than 2 n / C
+// each, and no row has more than its positions' grains)
 inline int paged_split_rows(const PagedParams& p) {
     return p.cap <= p.grain ? 0 : std::min(p.T, p.target / p.n_kv);
 }
-inline int paged_slots(const PagedParams& p) { return paged_split_rows(p) ? 2 * p.target / p.n_kv : 0; }
+inline int paged_slots(const PagedParams& p) {
+    if (!paged_split_rows(p)) return 0;
+    return (int)std::min((int64_t)(2 * p.target / p.n_kv), (int64_t)p.T * ((p.cap + p.grain - 1) / p.grain));
+}
 inline size_t paged_part_bytes(const PagedParams& p) {
     return (size_t)paged_slots(p) * p.n_kv * (p.rt * p.g) * (p.head_dim + 4) * 4;
 }

@@ -119,3 +119,17 @@ def test_workspace_holds_every_plan(n_kv, bf16):
             lens = [min(cap, C * rng.randint(1, 2) + 1) for _ in range(T)]
             C, chunks = _plan(lens, n_kv, grain)
     assert worst > 0.4  # the draws come near the bound
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_workspace_of_few_positions(bf16):
+    """A call needs no more partials than its rows' positions can have chunks, so a
+    few short rows do not hold what 1024 workgroups would."""
+    from ai_amd import _lib
+    L = _lib.lib()
+    grain = 128 if bf16 else 64
+    per_slot = 8 * 16 * (128 + 4) * 4
+    for T, pages in ((1, 1), (1, 16), (1, 17), (3, 40), (16, 64), (64, 8), (1, 4096), (64, 4096)):
+        a = _paged(kv_bf16=bf16, max_pages=pages, table_stride=pages)
+        chunks = T * -(-16 * pages // grain) if 16 * pages > grain else 0
+        assert L.rv12_paged_attend_workspace_bytes(ctypes.byref(a), T) == 16 + min(chunks, 256) * per_slot, (T, pages)
