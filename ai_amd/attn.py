@@ -112,6 +112,10 @@ class RopeAttn:
         check(rc, "prefill_rope_attn")
 
 
+_TOO_MANY = ("paged attention: at most 65536 rows, 2^30 positions in a table row, 2^35 of both multiplied and 2^40 times "
+             "n_kv")
+
+
 class PagedRopeAttn:
     """Attention over a cache of many sequences in pages (rv12_paged_append,
     rv12_paged_attend).  A pass has T token rows; row r is position pos[r] of
@@ -127,6 +131,9 @@ class PagedRopeAttn:
         table  int32 [sequences, pages of one], the page ids of each sequence
                (any stride between its rows)
         kc, vc [pages, n_kv, page, head_dim] of kv_dtype
+
+    At most 65536 rows and 2^30 positions in a row of the table; for attend, rows
+    times these at most 2^35 (and times n_kv 2^40: split a larger pass's rows).
 
     A row with seq or pos outside the table (-1 for padding a pass to a fixed
     size) is padding: its q and out are zeros and it writes nothing.  A page id
@@ -219,13 +226,16 @@ class PagedRopeAttn:
         with on(q.device):
             need = L.rv12_paged_attend_workspace_bytes(a, T)
             if need == 0:
-                raise ValueError("paged attention: too many rows or positions")
+                raise ValueError(_TOO_MANY)
             ws = torch.empty(need, dtype=torch.uint8, device=q.device)
             check(L.rv12_paged_attend(a, T, _ptr(q), _ptr(seq), _ptr(pos), _ptr(table), _ptr(kc), _ptr(vc), _ptr(out),
                                       _ptr(ws), need, _stream(q.device)), "paged_attend")
 
     def __call__(self, qkv, qn, kn, inv, seq, pos, table, kc, vc, out):
-        """append, then attend."""
+        """append, then attend (nothing is appended where attend would refuse)."""
+        n = pos.numel() * table.shape[-1] * self.page
+        if n > 1 << 35 or (n >> 10) * self.n_kv > 1 << 30:
+            raise ValueError(_TOO_MANY)
         q = torch.empty_like(out)
         self.append(qkv, qn, kn, inv, seq, pos, table, kc, vc, q)
         self.attend(q, seq, pos, table, kc, vc, out)

@@ -381,10 +381,11 @@ const char* rv12_strerror(int s) {
         case RV12_E_SCRATCH: return "workspace of the launch exceeds the static scratch (RV12_STATIC_SCRATCH_BYTES, 8 MiB)";
         case RV12_E_PAGED:
             return "bad paged cache or rows (head_dim 64 or 128, up to 16 query heads per kv head, pages of 16 .. 1024 "
-                   "positions in powers of two, T in [1, 65536], at most 2^30 positions in a table row)";
-        case RV12_E_RULES: return 
-            "bad logits or rules (T in [1, 65535], V in [1, 2^31 - 65536), fewer than 2^20 tokens and 2048 biases a row, "
-            "strides >= 0)";
+                   "positions in powers of two, T in [1, 65536], at most 2^30 positions in a table row; attention: T times "
+                   "those at most 2^35, and times the kv heads 2^40)";
+        case RV12_E_RULES:
+            return "bad logits or rules (T in [1, 65535], V in [1, 2^31 - 65536), fewer than 2^20 tokens and 2048 biases a "
+                   "row, strides >= 0)";
         case RV12_E_LORA:
             return "bad adapters (N >= 1, K % 32 == 0, rank a multiple of 8 up to 128, count >= 1) or T outside [1, 65536]";
         case RV12_E_LAUNCH: return "kernel launch failed";
@@ -814,9 +815,16 @@ static int paged_params(const rv12_paged* a, int t, PagedParams* p) {
     p->cap = cap;
     p->eps = a->eps;
     p->scale = a->scale;
-    // the plan's sum of 32-position blocks and its chunk length stay ints
-    if ((int64_t)t * cap > (int64_t)1 << 35 || (int64_t)t * cap / p->target * a->n_kv > (int64_t)1 << 30) return RV12_E_PAGED;
     p->grain = p->kv_bf16 ? 128 : 64;
+    return RV12_OK;
+}
+
+static int attend_params(const rv12_paged* a, int t, PagedParams* p) {
+    const int rc = paged_params(a, t, p);
+    if (rc) return rc;
+    // the plan's sum of 32-position blocks and its chunk length stay ints
+    const int64_t all = (int64_t)t * p->cap;
+    if (all > (int64_t)1 << 35 || all / p->target * p->n_kv > (int64_t)1 << 30) return RV12_E_PAGED;
     return RV12_OK;
 }
 
@@ -846,7 +854,7 @@ int rv12_paged_append(const rv12_paged* a, int t, const float* qkv, const float*
 
 size_t rv12_paged_attend_workspace_bytes(const rv12_paged* a, int t) {
     PagedParams p;
-    if (paged_params(a, t, &p)) return 0;
+    if (attend_params(a, t, &p)) return 0;
     return 16 + paged_plan_bytes(p) + paged_part_bytes(p);
 }
 
@@ -854,7 +862,7 @@ int rv12_paged_attend(const rv12_paged* a, int t, const float* q, const int32_t*
                       const int32_t* table, const void* kc, const void* vc, float* out, void* ws, size_t ws_bytes,
                       void* stream) {
     PagedParams p;
-    const int rc = paged_params(a, t, &p);
+    const int rc = attend_params(a, t, &p);
     if (rc) return rc;
     if (!q || !pos || !table || !kc || !vc || !out) return RV12_E_NULL;
     if (!aligned16(q) || !aligned16(kc) || !aligned16(vc) || !aligned16(out) || ((uintptr_t)pos & 7u) ||

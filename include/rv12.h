@@ -361,8 +361,8 @@ int rv12_prefill_rope_attn(const rv12_attn* a, int t, const float* qkv, const fl
  * graph can advance them.  A row whose sequence is outside [0, n_seq) or whose
  * position is outside [0, max_pages page) is padding.  A page id outside
  * [0, n_pages) is no page.  head_dim 64 or 128; n_heads / n_kv 1 .. 16; page a
- * power of two, 16 .. 1024; max_pages page at most 2^30, t max_pages page at most
- * 2^35 and times n_kv 2^40. */
+ * power of two, 16 .. 1024; max_pages page at most 2^30, and for the attention
+ * t max_pages page at most 2^35, times n_kv 2^40. */
 typedef struct rv12_paged {
     int32_t n_heads, n_kv, head_dim, page;
     int32_t kv_bf16; /* 1: bf16 caches, 0: float32 */

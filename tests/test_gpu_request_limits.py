@@ -87,6 +87,40 @@ def test_paged_head_counts_and_large_pages(H, KV, HD, page, kv):
 
 
 @pytest.mark.parametrize("kv", tp.KV_TYPES)
+def test_append_under_the_largest_table(kv):
+    """Rows up to the last of 2^30 positions, more of them than the attention takes
+    with such a table: appended alone, and refused before anything is written where
+    the attention is to follow."""
+    from ai_amd.attn import PagedRopeAttn
+    H, KV, HD, page, T = 4, 2, 64, 1024, 40
+    g = tp._gen(25)
+    table = torch.full((1, 1 << 20), -1, dtype=torch.int32, device="cuda")
+    pos = torch.cat([torch.arange(20), torch.arange((1 << 30) - 20, 1 << 30)]).cuda()
+    table[0, 0], table[0, -1] = 2, 0
+    kc, vc = (tp._randn(g, 3, KV, page, HD).to(kv) for _ in range(2))
+    kc0, vc0 = kc.clone(), vc.clone()
+    qkv, ones, seq = tp._randn(g, T, (H + 2 * KV) * HD), torch.ones(HD, device="cuda"), torch.zeros(T, dtype=torch.int32).cuda()
+    p = PagedRopeAttn(H, KV, HD, page, kv, tp.EPS)
+    q, out = torch.full((T, H * HD), float("nan"), device="cuda"), torch.zeros(T, H * HD, device="cuda")
+    args = (qkv, ones, ones, tp._inv(HD), seq, pos, table, kc, vc)
+    for call in (lambda: p(*args, out), lambda: p.attend(q, seq, pos, table, kc, vc, out)):
+        with pytest.raises(ValueError):
+            call()
+    torch.cuda.synchronize()
+    assert torch.equal(kc, kc0) and torch.equal(vc, vc0)
+    p.append(*args, q)
+    torch.cuda.synchronize()
+    rq, rk, rv, bq, bk = tp._append_ref(qkv, ones, ones, tp._inv(HD), pos, H, KV, HD)
+    assert bool(((q.double().view(T, H, HD) - rq).abs() <= bq).all())
+    pid, at = torch.tensor([2] * 20 + [0] * 20, device="cuda"), pos % page
+    half = torch.finfo(kv).eps / 2
+    assert torch.equal(vc[pid, :, at], rv.to(kv))
+    assert bool(((kc[pid, :, at].double() - rk).abs() <= bk + half * (rk.abs() + bk)).all())
+    kc0[pid, :, at], vc0[pid, :, at] = kc[pid, :, at], vc[pid, :, at]
+    assert torch.equal(kc, kc0) and torch.equal(vc, vc0)  # and nowhere else
+
+
+@pytest.mark.parametrize("kv", tp.KV_TYPES)
 def test_graph_of_more_than_64_rows(kv):
     """A captured pass of 150 rows (its plan a launch of its own) replayed with other
     rows each time, beside a second graph of the same object, and eager calls."""

@@ -133,3 +133,20 @@ def test_workspace_of_few_positions(bf16):
         a = _paged(kv_bf16=bf16, max_pages=pages, table_stride=pages)
         chunks = T * -(-16 * pages // grain) if 16 * pages > grain else 0
         assert L.rv12_paged_attend_workspace_bytes(ctypes.byref(a), T) == 16 + min(chunks, 256) * per_slot, (T, pages)
+
+
+def test_rows_times_positions_bounds_the_attention_alone():
+    """The plan's sums hold 2^35 row positions (2^40 times the kv heads); the append
+    has no plan, and takes as many rows as any table."""
+    from ai_amd import _lib
+    L = _lib.lib()
+    p = 4096
+    for T, pages, n_kv, fits in ((32, 1 << 20, 8, True), (33, 1 << 20, 8, False), (65536, 512, 8, True), (65536, 513, 8, False),
+                                 (32, 1 << 20, 32, True), (32, 1 << 20, 33, False), (65536, 1 << 20, 256, False)):
+        a = _paged(n_heads=n_kv, n_kv=n_kv, page=1024, max_pages=pages, table_stride=pages)
+        assert (L.rv12_paged_attend_workspace_bytes(ctypes.byref(a), T) > 0) == fits, (T, pages, n_kv)
+        rc = L.rv12_paged_attend(ctypes.byref(a), T, p, p, p, p, p, p, p, None, 1 << 50, None)
+        assert rc == (_lib.RV12_E_WORKSPACE if fits else _lib.RV12_E_PAGED)
+        # past the size checks: the next one is for the pointers
+        assert L.rv12_paged_append(ctypes.byref(a), T, None, p, p, p, p, p, p, p, p, p, None) == _lib.RV12_E_NULL
+    assert "2^35" in _lib.strerror(_lib.RV12_E_PAGED)
