@@ -897,8 +897,8 @@ int rv12_logits_adjust(const rv12_rules* rules, const float* x, int64_t x_stride
     if (!rules || !x || !y) return RV12_E_NULL;
     const rv12_rules& a = *rules;
     if (!rv12_logits_workspace_bytes(v, t)) return RV12_E_RULES;
-    if (a.max_tokens < 0 || a.max_tokens >= 1 << kAdjustCountBits || a.n_bias < 0 || a.n_bias > 2047 || a.tokens_stride < 0 || a.bias_stride < 0 || a.mask_stride < 0 ||
-        x_stride < 0 || (t > 1 && y_stride < v))
+    if (a.max_tokens < 0 || a.max_tokens >= 1 << kAdjustCountBits || a.n_bias < 0 || a.n_bias > 2047 ||
+        a.tokens_stride < 0 || a.bias_stride < 0 || a.mask_stride < 0 || x_stride < 0 || (t > 1 && y_stride < v))
         return RV12_E_RULES;
     if (a.tokens && (!a.length || !a.penalties)) return RV12_E_NULL;
     if (a.n_bias && (!a.bias_ids || !a.bias)) return RV12_E_NULL;

@@ -13,9 +13,11 @@
 // straight from memory), B operand column l % 16 (the token), result rows
 // 4 (l / 16) + 0..3.
 //
-// A prompt is bound by y and out (2051 rows beside 24576 outputs, rank 64: 448 MB in
-// 15 + 93 us, 4.2 TB/s); a few rows by two launches of dependent round trips (4 + 5
-// us for one row, 7 + 7 for 16 of 13 adapters).
+// A prompt is bound by its bytes (rank 64, 2051 rows of 4096 beside 24576 outputs, y
+// and out: 448 MB in 15 + 93 us, 4.2 TB/s; behind the gate, 2 x 12288 beside 4096, x:
+// the 138 MB of the 1368 rows with an adapter in 45 us, 3.1 TB/s, then 28); a few rows
+// by two launches of dependent round trips (4 + 5 us for one row, 7 + 7 for 16 of 13
+// adapters).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

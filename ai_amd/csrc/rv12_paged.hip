@@ -166,9 +166,14 @@ void launch_paged_append(const PagedParams& p, hipStream_t st) {
 // chunk order.
 //
 // Bound by the cache's bytes once they are many: 64 rows of 500 to 8200 positions,
-// 32 heads over 8, bf16, 730 MB in 134 us (5.4 TB/s) and the join in 6; 32771
-// positions of one row 26 + 4 us.  A few short rows take 6 us of dependent
-// round trips (rows, table, keys, values, the join in LDS) and 3-4 us for the join.
+// 32 heads over 8, bf16, 730 MB in 130 us (5.6 TB/s) and the join in 6; 32771
+// positions of one row 25 + 4 us.  One row of 16 positions takes 6.2 us, all of it
+// dependent round trips (rows, table, keys, values, the join in LDS); 8 float32 rows
+// of 60 to 700 positions, 16 heads over 8, take that, 3.8 for their 18 MB, and 4 in
+// the join's own launch: 10.3 + 4.  A prompt of 2048 rows, 32 heads over 8, takes 187 us
+// in bf16 and 361 in float32, the plan's 7 and the join's 5 among them: 34 GFLOP, in
+// bf16 in three parts each, that keep the matrix cores busy 22 % of the time; the
+// waves wait a third of theirs.
 
 // the rows r = base + lane of a plan step: leader rows have the number of rows
 // they lead (nr) and the positions to cover (n, 0 for a padding row); key: the row's
@@ -232,11 +237,11 @@ __device__ __forceinline__ PlanRows plan_rows(const PagedParams& p, int base) {
 
 // chunk length of the plan over `total` blocks of 32 positions
 __device__ __forceinline__ int plan_chunk(const PagedParams& p, int total) {
-    // up to 512 positions a chunk's own cost counts, and one workgroup per
-    // resident slot is best; above it smaller chunks even out the workgroups' ends
-    // (1024 target: 8 rows of one sequence at 4096 positions, 64 query heads over 8,
-    // 18.9 -> 16.9 us with half the workgroups; 64 rows of 500 to 8200 positions, 32
-    // heads over 8, 142 us, 155 with half)
+    // up to 512 positions a chunk's own cost (its round trips, its partials) counts,
+    // and two workgroups per CU are best; above it smaller chunks even out the
+    // workgroups' ends (both passes, us with the target's workgroups and with half of
+    // them: 8 rows of one sequence at 4104 positions, 64 query heads over 8, 25.3,
+    // 21.7; 64 rows of 500 to 8200 positions, 32 heads over 8, 141, 156)
     const int64_t all = (int64_t)total * p.n_kv;
     constexpr int64_t kKnee = 512;
     const int64_t half_c = (all + p.target / 2 - 1) / (p.target / 2) * 32;
@@ -284,7 +289,7 @@ __device__ __forceinline__ bool plan_find(const PagedParams& p, int want, PlanIt
 // rows of several chunks), then every item, then the rows of several chunks.  The
 // waves take the steps of 64 rows in turn, in three passes over them: the sum of
 // the positions, the numbers of items and slots, the entries.  (Worked out in every
-// workgroup, as for up to 64 rows, a prompt of 2048 rows took 850 us, not 206.)
+// workgroup, as for up to 64 rows, a prompt of 2048 rows took 850 us in all, not 187.)
 constexpr int kPlanThreads = 1024;
 __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PagedParams p) {
     constexpr int NW = kPlanThreads / 64;

@@ -29,7 +29,8 @@ def _vector(t, name, dtype, T, dev):
 def adjust(x, out=None, tokens=None, length=None, prompt=None, penalties=None, bias_ids=None, bias=None, mask=None,
            ids=None):
     """The rules on the logits x (float32 [T, V]) into out (None: in place; a given
-    out is x or does not overlap it), which is returned.  Per row and id n, in float32 and this order:
+    out is x or does not overlap it), which is returned.  Per row and id n, in
+    float32 and this order:
 
         n among the row's tokens:            l = l / repetition if l > 0 else l * repetition
         n generated c > 0 times:             l -= frequency * c + presence
@@ -48,8 +49,10 @@ def adjust(x, out=None, tokens=None, length=None, prompt=None, penalties=None, b
                smallest on ties, NaN counting as the largest, -1 where the mask
                allows none
 
-    L is below 2^20 and M below 2^11.  Ids outside [0, V), such as the -1 of an unused entry, are passed over.  All on
-    one GPU; nothing is read back, so a call can be captured in a HIP graph."""
+    T is at most 65535, V below 2^31 - 65536, L below 2^20 (whatever the lengths) and
+    M below 2^11.  Ids outside [0, V), such as the -1 of an unused entry, are passed
+    over.  All on one GPU; nothing is read back, so a call can be captured in a HIP
+    graph."""
     if not torch.is_tensor(x) or not x.is_cuda:
         raise ValueError("adjust: x must be a tensor on the GPU")
     if x.dim() != 2 or x.shape[1] < 1:

@@ -71,13 +71,14 @@ class Adapters:
         return cls(A, B, scale, [a.shape[0] for a, _, _ in pairs])
 
     def apply(self, x, y, idx, mode=0, lnw=None, eps=1e-6, out=None):
-        """out[t] = y[t] + scale B (A x'[t]) of adapter idx[t], for the T rows of
-        x; out None: into y; a given out is y or does not overlap it.  mode, lnw and eps give x' as the shared linear's
-        call has it (wcomp.gemvc1): modes 0 and 1 x' = x (float32 [T, K]), with
-        lnw (bf16 [K]) its RMSNorm; mode 2 x' = silu(x[:, :K]) * x[:, K:].  idx:
-        int32 [T], outside [0, count) (-1) no adapter: out[t] = y[t].  y and out:
-        float32 [T, N], rows contiguous, any stride between them (a slice of a
-        fused projection's output).  Can be captured in a HIP graph."""
+        """out[t] = y[t] + scale B (A x'[t]) of adapter idx[t], for the T <= 65536
+        rows of x; out None: into y; a given out is y or does not overlap it.  mode,
+        lnw and eps give x' as the shared linear's call has it (wcomp.gemvc1): modes
+        0 and 1 x' = x (float32 [T, K]), with lnw (bf16 [K]) its RMSNorm; mode 2
+        x' = silu(x[:, :K]) * x[:, K:].  idx: int32 [T], outside [0, count) (-1) no
+        adapter: out[t] = y[t].  y and out: float32 [T, N], rows contiguous, any
+        stride between them (a slice of a fused projection's output).  Can be
+        captured in a HIP graph."""
         dev, K, N = self._index, self.K, self.N
         if mode not in (0, 1, 2):
             raise ValueError("apply: mode must be 0, 1 or 2")

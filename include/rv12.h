@@ -417,8 +417,8 @@ int rv12_paged_attend(const rv12_paged* a, int t, const float* q, const int32_t*
  * repetition, frequency, presence (NULL with tokens NULL); bias_ids / bias: n_bias
  * entries per row; mask: bit n & 31 of word n >> 5 of the row set where id n is
  * allowed.  Ids outside [0, v) in tokens and bias_ids are passed over.  Every
- * part may be absent (NULL).  max_tokens below 2^20, n_bias below 2^11.  Strides are in elements, from row to row.  A field's
- * rows may all be one (stride 0). */
+ * part may be absent (NULL).  max_tokens below 2^20, n_bias below 2^11.  Strides
+ * are in elements, from row to row.  A field's rows may all be one (stride 0). */
 typedef struct rv12_rules {
     const int64_t* tokens;
     const int32_t* length;
@@ -432,9 +432,10 @@ typedef struct rv12_rules {
 } rv12_rules;
 
 /* y[r] = the rules on x[r], 1 <= t <= 65535 rows of 1 <= v < 2^31 - 65536 logits
- * (y may be x: each logit is read and written once; else the two do not overlap).  ids: NULL, or int64[t] that
- * receives the id of each row's largest y among the allowed ones, the smallest on
- * ties, NaN counting as larger than any number, -1 where the mask allows none.
+ * (y may be x: each logit is read and written once; else the two do not overlap).
+ * ids: NULL, or int64[t] that receives the id of each row's largest y among the
+ * allowed ones, the smallest on ties, NaN counting as larger than any number, -1
+ * where the mask allows none.
  * ws: rv12_logits_workspace_bytes(v, t) bytes, 8-byte aligned, read only with ids.
  * Stands beside rv12_head_argmax (the pick without rules); the reference applies
  * its grammar masks on the host
@@ -460,9 +461,10 @@ typedef struct rv12_lora {
  * x (rows k floats apart, 2 k in mode 2) and x' as rv12_gemv: mode 0 or 1 x' = x,
  * with lnw the RMSNorm; mode 2 x' = silu(x[0:k]) * x[k:2k] (no lnw).  A row whose
  * idx is outside [0, count) has no adapter: out[i] = y[i].  out may be y (same
- * stride), else the two do not overlap; strides in floats.  Products of x', a, b and the sums between are
- * float32 exact to rounding (three bf16 parts), finite x assumed.  Two passes, no
- * atomics.  ws: rv12_lora_workspace_bytes(r, k, t) bytes, 16-byte aligned. */
+ * stride), else the two do not overlap; strides in floats.  Products of x', a, b and
+ * the sums between are float32 exact to rounding (three bf16 parts), finite x
+ * assumed.  Two passes, no atomics.  ws: rv12_lora_workspace_bytes(r, k, t) bytes,
+ * 16-byte aligned. */
 size_t rv12_lora_workspace_bytes(int r, int k, int t);
 int rv12_lora_apply(const rv12_lora* a, const float* x, const float* y, int64_t y_stride, float* out, int64_t out_stride,
                     const int32_t* idx, int t, const uint16_t* lnw, float eps, int mode, void* ws, size_t ws_bytes,
