@@ -139,11 +139,11 @@ class PagedRopeAttn:
     size) is padding: its q and out are zeros and it writes nothing.  A page id
     outside the cache (-1) is no page: its positions take no part in the
     attention, a key or value for it is dropped.  A row that sees an infinite key
-    or value may be NaN.  Rows that name one slot
-    together leave it with either's key and value.  seq, pos and table are read
-    on the device, so a call can be captured in a HIP graph; every call has a
-    workspace of its own.  The rotation angle is formed in 64 bits (RopeAttn's
-    in float32: the two agree to float32 rounding times the position)."""
+    or value may be NaN.  Rows that name one slot together leave it with either's
+    key and value.  seq, pos and table are read on the device, so a call can be
+    captured in a HIP graph; every call has a workspace of its own.  The rotation
+    angle is formed in 64 bits (RopeAttn's in float32: the two agree to float32
+    rounding times the position)."""
 
     def __init__(self, n_heads, n_kv, head_dim, page, kv_dtype, eps, scale=None):
         if kv_dtype not in (torch.float32, torch.bfloat16):
@@ -233,7 +233,7 @@ class PagedRopeAttn:
 
     def __call__(self, qkv, qn, kn, inv, seq, pos, table, kc, vc, out):
         """append, then attend (nothing is appended where attend would refuse)."""
-        n = pos.numel() * table.shape[-1] * self.page
+        n = pos.numel() * table.shape[-1:].numel() * self.page
         if n > 1 << 35 or (n >> 10) * self.n_kv > 1 << 30:
             raise ValueError(_TOO_MANY)
         q = torch.empty_like(out)

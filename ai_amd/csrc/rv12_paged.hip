@@ -27,7 +27,7 @@ namespace rv12 {
 //
 // Bound by bytes (4 (H + 2 KV) HD read, 4 H HD + 2 KV HD EB written per row: 4099
 // rows of 32 heads over 8 take 37 us into bf16 pages, 5.0 TB/s, and 42 into float32
-// ones, 4.8: the rate of a copy); at a few rows by its latency (2.5 us for one, 3.5
+// ones, 4.8: the rate of a copy); at a few rows by its latency (2.2 us for one, 3.3
 // for 64).  HD / 8 lanes hold a head, 4 consecutive dims of either rotation half
 // each, so every access is 16 bytes (8 where bf16 is stored) and the norm's sum
 // stays within 16 lanes.  A workgroup of 256 threads takes a share of one row's
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedParams p) {
 }
 
 void launch_paged_append(const PagedParams& p, hipStream_t st) {
-    // a row's heads in one or more workgroups, a head each for its LPH threads
+    // a thread group for every head of a row
     const int slots = 256 / (p.head_dim / 8), nh = p.n_heads + 2 * p.n_kv;
     const dim3 grid((unsigned)p.T, (unsigned)((nh + slots - 1) / slots));
     if (p.head_dim == 128) {

@@ -150,3 +150,15 @@ def test_rows_times_positions_bounds_the_attention_alone():
         # past the size checks: the next one is for the pointers
         assert L.rv12_paged_append(ctypes.byref(a), T, None, p, p, p, p, p, p, p, p, p, None) == _lib.RV12_E_NULL
     assert "2^35" in _lib.strerror(_lib.RV12_E_PAGED)
+
+
+def test_call_refuses_shapeless_tables():
+    """append and attend in one call look at the table's size first: a table of no
+    dimension is refused as by append."""
+    from ai_amd.attn import PagedRopeAttn
+    p = PagedRopeAttn(8, 4, 64, 16, torch.float32, 1e-6)
+    z = torch.zeros
+    pos = z(1, dtype=torch.int64)
+    for table in (torch.tensor(0, dtype=torch.int32), z(3, dtype=torch.int32), z(0, 0, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            p(z(1, 1024), z(64), z(64), z(32), None, pos, table, z(1, 4, 16, 64), z(1, 4, 16, 64), z(1, 512))
